@@ -20,7 +20,7 @@ class df_status_t(ctypes.Structure):
                 ("block", ctypes.c_uint32), ("aux", ctypes.c_uint32)]
 
 
-_vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_vp, _i, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
 
 MAX_WORLD = 8
 MAX_CTAS = 64
@@ -93,6 +93,8 @@ SIGNATURES: dict[str, tuple] = {
     "df_kv_cache_append_bf16": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
     "df_small_gemm_plan": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "df_rope_append_bf16": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp]),
+    "df_page_plan": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    "df_rope_append_paged4_bf16": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp]),
     "df_mlp_gated_bf16_static": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

@@ -16,8 +16,9 @@ import torch
 from . import _native
 from ._native import df_status_t
 
-DEVICE_ERRORS = {1: "DF_ERR_TIMEOUT", 2: "DF_ERR_PEER"}
-_WHERE = {1: "tma-producer", 2: "mma(full)", 3: "mma(tmem-empty)", 4: "epilogue", 5: "h-ready", 16: "peer-flag", 21: "small-gemm-producer", 22: "small-gemm-mma", 23: "small-gemm-epilogue", 24: "small-gemm-partial-rows", 32: "attention-producer", 33: "attention-mma", 34: "attention-softmax"}
+DEVICE_ERRORS = {1: "DF_ERR_TIMEOUT", 2: "DF_ERR_PEER", 3: "DF_ERR_PLAN"}
+_WHERE = {1: "tma-producer", 2: "mma(full)", 3: "mma(tmem-empty)", 4: "epilogue", 5: "h-ready", 16: "peer-flag", 21: "small-gemm-producer", 22: "small-gemm-mma", 23: "small-gemm-epilogue", 24: "small-gemm-partial-rows", 32: "attention-producer", 33: "attention-mma", 34: "attention-softmax",
+          48: "page-plan(pages missing)", 49: "page-plan(table row full)", 50: "page-plan(rows missing)"}
 
 
 class DeviceStatusError(RuntimeError):
@@ -89,6 +90,32 @@ def _stream_ptr(t: torch.Tensor) -> int:
 def _check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed ({rc}): {_native.last_error()}")
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the CUDA device that all the tensors are on."""
+    idx = _dev_index(first)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
+    return idx
+
+
+def _launch(idx: int, what: str, *args) -> None:
+    """Calls an entry point with the tensors' device current (launches go to the current device)."""
+    fn = getattr(_native.load(), what)
+    if torch.cuda.current_device() == idx:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args)
+    if rc != 0:
+        _check(rc, what)
+
+
+def _require_int32(name: str, t: torch.Tensor, *shape: int) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _require_bf16_2d(name: str, t: torch.Tensor) -> None:
@@ -327,4 +354,90 @@ def gated_mlp_static(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, 
     rc = _native.load().df_mlp_gated_bf16_static(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                                                  out.data_ptr(), M, H, I, max_ctas, st.data_ptr(), _stream_ptr(x))
     _check(rc, "df_mlp_gated_bf16_static")
+    return out
+
+
+# ------------------------------------------------------ paged 4-bit key/value cache
+PAGE_GRANULE = 16          # page sizes are multiples of this many tokens
+PAGED4_TOKEN_BYTES = 136   # one token of one key/value head: 64 bytes of codes and 4 of parameters, for key and value
+
+
+def paged4_cache(num_pages: int, kv_heads: int, page_size: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """One layer's cache, ``uint8 [num_pages, kv_heads, page_size * 136]`` (contents arbitrary: only slots that were
+    written are read)."""
+    if num_pages <= 0 or kv_heads <= 0 or page_size <= 0 or page_size % PAGE_GRANULE:
+        raise ValueError(f"num_pages and kv_heads must be positive, page_size a multiple of {PAGE_GRANULE}")
+    return torch.empty(num_pages, kv_heads, page_size * PAGED4_TOKEN_BYTES, dtype=torch.uint8, device=device)
+
+
+def _require_paged4(cache: torch.Tensor, page_size: int) -> None:
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or page_size <= 0 \
+            or page_size % PAGE_GRANULE or cache.shape[2] != page_size * PAGED4_TOKEN_BYTES:
+        raise ValueError(f"expected a contiguous uint8 cache [pages, kv_heads, page_size * {PAGED4_TOKEN_BYTES}], page_size a "
+                         f"multiple of {PAGE_GRANULE}; got {cache.dtype} {tuple(cache.shape)} and page_size {page_size}")
+
+
+def page_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.Tensor, page_counts: torch.Tensor,
+              free_pages: torch.Tensor, free_count: torch.Tensor, row_starts: torch.Tensor, slots: torch.Tensor,
+              positions: torch.Tensor, *, page_size: int, rows_per_request: int = 0) -> None:
+    """Page tables, slots and positions of a step, on the device (``df_page_plan``): request ``b`` is ``seq_lens[b]`` tokens
+    long after the step, ``new_lens[b]`` of them new. Updates ``page_table [B, max_pages]``, ``page_counts [B]`` and the free
+    list ``free_pages [num_pages]`` / ``free_count [1]`` (pages no longer needed are given back first, so length 0 ends a
+    request); writes ``row_starts [B + 1]`` and, per row, ``slots`` and ``positions`` (``-1`` and 0 where there is no token).
+    ``rows_per_request`` 0: new tokens back to back; else request ``b`` owns rows ``b * rows_per_request ...``. All int32.
+    Too few free pages, a full table row or too few rows are reported by ``check_status``."""
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [requests, max_pages], got {tuple(page_table.shape)}")
+    B, max_pages = page_table.shape
+    _require_int32("page_table", page_table, B, max_pages)
+    _require_int32("seq_lens", seq_lens, B)
+    _require_int32("new_lens", new_lens, B)
+    _require_int32("page_counts", page_counts, B)
+    _require_int32("free_pages", free_pages, free_pages.numel())
+    _require_int32("free_count", free_count, 1)
+    _require_int32("row_starts", row_starts, B + 1)
+    rows = slots.numel()
+    _require_int32("slots", slots, rows)
+    _require_int32("positions", positions, rows)
+    if B == 0:
+        raise ValueError("page_plan needs at least one request")
+    idx = _same_device(page_table, seq_lens, new_lens, page_counts, free_pages, free_count, row_starts, slots, positions)
+    _launch(idx, "df_page_plan", seq_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), page_counts.data_ptr(),
+            free_pages.data_ptr(), free_count.data_ptr(), row_starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), B,
+            max_pages, free_pages.numel(), rows, page_size, rows_per_request, status_block(page_table.device).data_ptr(),
+            _stream_ptr(page_table))
+
+
+def rope_angles(num_positions: int, theta: float, device: torch.device | str = "cuda") -> torch.Tensor:
+    """``[num_positions, 128]`` fp32: cos, then sin, of the 64 rotary angles of every position (formed in 64 bits: a
+    32-bit angle of a far position is off by more than a bf16 step)."""
+    freq = theta ** (-torch.arange(64, dtype=torch.float64, device=device) / 64)
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, angles: torch.Tensor, q_heads: int,
+                       kv_heads: int, cache: torch.Tensor, *, page_size: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary embedding of the query and key heads of ``qkv [rows, (Hq + 2 Hkv) * 128]`` at ``positions``, keys and values
+    quantised into the ``slots`` of a paged 4-bit cache, one launch. ``out`` (default: in place) receives the rotated queries,
+    and keys and values as the cache stands for them, so that attention over these rows sees what later steps will see.
+    Rows with a slot or position out of range are padding: left as they are in ``out``. ``angles`` from ``rope_angles``."""
+    _require_bf16_2d("qkv", qkv)
+    _require_paged4(cache, page_size)
+    out = qkv if out is None else out
+    if out is not qkv:
+        _require_bf16_2d("out", out)
+    rows = qkv.shape[0]
+    if qkv.shape[1] != (q_heads + 2 * kv_heads) * 128 or tuple(out.shape) != tuple(qkv.shape) or cache.shape[1] != kv_heads:
+        raise ValueError("expected qkv and out [rows, (q_heads + 2 kv_heads) * 128] and a cache of kv_heads heads")
+    if angles.dtype != torch.float32 or angles.dim() != 2 or angles.shape[1] != 128 or not angles.is_contiguous():
+        raise ValueError("angles must be a contiguous fp32 tensor [positions, 128]")
+    _require_int32("positions", positions, rows)
+    _require_int32("slots", slots, rows)
+    idx = _same_device(qkv, positions, slots, angles, cache, out)
+    if rows == 0:
+        return out
+    _launch(idx, "df_rope_append_paged4_bf16", qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), positions.data_ptr(),
+            slots.data_ptr(), angles.data_ptr(), angles.shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), cache.shape[0],
+            page_size, _stream_ptr(qkv))
     return out

@@ -41,6 +41,12 @@ extern "C" {
 #define DF_ERR_NONE 0u
 #define DF_ERR_TIMEOUT 1u /* a bounded wait ran past the deadline */
 #define DF_ERR_PEER 2u    /* a peer rank never raised its flag     */
+#define DF_ERR_PLAN 3u    /* df_page_plan: a request could not be given what it asked for */
+
+/* df_status_t.where of DF_ERR_PLAN */
+#define DF_WHERE_PLAN_PAGES 48u /* free list too short (aux: pages missing); no request was given pages */
+#define DF_WHERE_PLAN_TABLE 49u /* request aux needs more pages than a row of the table has; it keeps what it holds */
+#define DF_WHERE_PLAN_ROWS 50u  /* more new tokens than rows; the last ones have no row */
 
 /* Asynchronous device status block (16 bytes of device memory, zero = ok). */
 typedef struct df_status {
@@ -460,6 +466,45 @@ int df_rope_append_bf16(void* qkv, int row_stride, const int* seq_lens_dev, int 
  *     through df_mlp_gated_bf16. */
 int df_mlp_gated_bf16_static(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* out,
                              int M, int H, int I, int max_ctas, df_status_t* dev_status, void* stream);
+
+/* ------------------------------------------- key/value cache in pages of 4-bit codes
+ *
+ * The cache of one layer is uint8 [num_pages, kv_heads, page_size * 136]; page_size is a multiple of 16, the head
+ * dimension 128. 16 tokens of a head are one granule of 2176 bytes: key codes [16][64] (byte i of a token holds
+ * dimensions 2i, low four bits, and 2i + 1; 16-byte chunk c of token r is stored at place c ^ ((r >> 1) & 3)), key
+ * parameters [16][2] in bf16 (scale, minimum), then the same for the values. A code n stands for scale * n + minimum.
+ * Token `pos` of a request lives in page page_table[request][pos / page_size]; its slot is
+ * page * page_size + pos % page_size. The reference leaves the cache to the host engine
+ * (examples/ae/scheduler/vllm/nanoflow.py:91-94, 231); these entry points are what an attention-tagged subgraph is
+ * substituted with when the cache is paged. */
+
+/* Brings the page tables in line with the requests' lengths and lays out the step's rows; all arguments are device
+ * memory, int32. Request b is seq_lens[b] tokens long AFTER this step, new_lens[b] of them are new; it needs
+ * ceil(seq_lens[b] / page_size) pages and holds page_counts[b] (updated), listed in page_table[b][0 ..). Pages it no
+ * longer needs go back on top of the free list (free_pages[0 .. free_count), updated; the free list has num_pages
+ * entries), then missing ones are taken from its top, requests in order; a step that is taken back (the former
+ * lengths, new_lens zero) restores the list exactly. A finished request has length 0. Entries of the table past
+ * page_counts[b] are written -1 when a page leaves.
+ * Rows: with rows_per_request == 0 the new tokens of all requests lie back to back, else request b's are rows
+ * b * rows_per_request ...; row_starts [requests + 1] receives where each begins, slots and positions [rows] the slot
+ * and the position of every row (-1 and 0 for rows without a token, and -1 for a token whose page is missing).
+ * If the free list does not hold enough pages, no request is given any and dev_status receives DF_ERR_PLAN (also for
+ * a request that outgrows its table row, and for too few rows). At most 8192 requests. Deterministic. */
+int df_page_plan(const int* seq_lens_dev, const int* new_lens_dev, int* page_table_dev, int* page_counts_dev,
+                 int* free_pages_dev, int* free_count_dev, int* row_starts_dev, int* slots_dev, int* positions_dev,
+                 int requests, int max_pages, int num_pages, int rows, int page_size, int rows_per_request,
+                 df_status_t* dev_status, void* stream);
+
+/* Rotary embedding of the query and key heads of `rows` fused rows [q heads | k heads | v heads], keys and values
+ * quantised into the slots of the cache, in one launch. angles [num_positions][128] fp32: cos then sin of the 64
+ * angles of a position; the rotated value is rounded to bf16. Per token and head: scale = bf16(max / 15 - min / 15),
+ * code = round-half-even((x - min) / scale) limited to 0 .. 15 (scale 0: code 0). `out` (may be qkv itself) receives
+ * the rotated queries, and keys and values as the cache stands for them, rounded to bf16. A row whose slot is outside
+ * [0, num_pages * page_size) or whose position is outside the table is padding and left as it was in `out`; two rows
+ * must not have the same slot. Strides in elements. */
+int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, void* out, long long ld_out, const int* positions_dev,
+                               const int* slots_dev, const float* angles_dev, int num_positions, int rows, int q_heads,
+                               int kv_heads, int head_dim, void* cache, int num_pages, int page_size, void* stream);
 
 #ifdef __cplusplus
 }
