@@ -95,6 +95,9 @@ SIGNATURES: dict[str, tuple] = {
     "df_rope_append_bf16": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp]),
     "df_page_plan": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     "df_rope_append_paged4_bf16": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp]),
+    "df_attention_paged4_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "df_attention_paged4_bf16": (_i, [_vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                                      _sz, _i, _vp, _vp]),
     "df_mlp_gated_bf16_static": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

@@ -18,7 +18,8 @@ from ._native import df_status_t
 
 DEVICE_ERRORS = {1: "DF_ERR_TIMEOUT", 2: "DF_ERR_PEER", 3: "DF_ERR_PLAN"}
 _WHERE = {1: "tma-producer", 2: "mma(full)", 3: "mma(tmem-empty)", 4: "epilogue", 5: "h-ready", 16: "peer-flag", 21: "small-gemm-producer", 22: "small-gemm-mma", 23: "small-gemm-epilogue", 24: "small-gemm-partial-rows", 32: "attention-producer", 33: "attention-mma", 34: "attention-softmax",
-          48: "page-plan(pages missing)", 49: "page-plan(table row full)", 50: "page-plan(rows missing)"}
+          48: "page-plan(pages missing)", 49: "page-plan(table row full)", 50: "page-plan(rows missing)",
+          51: "paged-attention"}
 
 
 class DeviceStatusError(RuntimeError):
@@ -440,4 +441,56 @@ def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.
     _launch(idx, "df_rope_append_paged4_bf16", qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), positions.data_ptr(),
             slots.data_ptr(), angles.data_ptr(), angles.shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), cache.shape[0],
             page_size, _stream_ptr(qkv))
+    return out
+
+
+def attention_paged4_workspace(requests: int, q_heads: int, kv_heads: int, max_new: int = 1,
+                               device: torch.device | str = "cuda") -> torch.Tensor:
+    """Scratch for ``attention_paged4`` (partial results of cut requests); its contents are arbitrary. Calls that can overlap
+    on the GPU, captured graphs included, need one each."""
+    need = int(_native.load().df_attention_paged4_workspace_bytes(requests, q_heads, kv_heads, max_new))
+    if need == 0:
+        raise ValueError("requests, max_new and the head counts must be positive, q_heads a multiple of kv_heads")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, out: torch.Tensor,
+                     workspace: torch.Tensor, *, page_size: int, row_starts: torch.Tensor | None = None,
+                     new_lens: torch.Tensor | None = None, max_new: int = 1, scale: float | None = None,
+                     max_ctas: int = 0) -> torch.Tensor:
+    """The new tokens' attention over a paged 4-bit cache. ``q, out [rows, Hq * 128]`` (2-D bf16 views, unit inner stride),
+    ``cache [pages, Hkv, page_size * 136]``, ``page_table [B, max_pages]`` and ``seq_lens [B]`` int32. Without ``new_lens``
+    row ``b`` is request ``b``'s one new token; with ``row_starts [B + 1]`` and ``new_lens [B]`` (from ``page_plan``) request ``b``
+    has rows ``row_starts[b] ...``, at most ``max_new``, causal among themselves. Rows of no request keep what they held, a row
+    without keys is zeros."""
+    _require_bf16_2d("q", q)
+    _require_bf16_2d("out", out)
+    _require_paged4(cache, page_size)
+    hd = 128
+    rows, cols = q.shape
+    kv_heads = cache.shape[1]
+    if cols == 0 or cols % (hd * kv_heads) or tuple(out.shape) != (rows, cols):
+        raise ValueError("expected q/out [rows, Hq * 128], Hq a multiple of the cache's heads")
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [requests, max_pages], got {tuple(page_table.shape)}")
+    B, max_pages = page_table.shape
+    _require_int32("page_table", page_table, B, max_pages)
+    _require_int32("seq_lens", seq_lens, B)
+    if (row_starts is None) != (new_lens is None):
+        raise ValueError("row_starts and new_lens come together")
+    if new_lens is not None:
+        _require_int32("row_starts", row_starts, B + 1)
+        _require_int32("new_lens", new_lens, B)
+    elif max_new != 1 or rows < B:
+        raise ValueError("without new_lens every request has one row: max_new must be 1, q at least as many rows as requests")
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor")
+    idx = _same_device(q, cache, page_table, seq_lens, out, workspace, row_starts, new_lens)
+    if rows == 0 or B == 0:
+        return out
+    _launch(idx, "df_attention_paged4_bf16", q.data_ptr(), q.stride(0), cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+            None if row_starts is None else row_starts.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
+            out.data_ptr(), out.stride(0), rows, B, max_pages, cache.shape[0], page_size, cols // hd, kv_heads, hd, max_new,
+            hd ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), max_ctas,
+            status_block(q.device).data_ptr(), _stream_ptr(q))
     return out

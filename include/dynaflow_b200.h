@@ -506,6 +506,20 @@ int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, void* out, lon
                                const int* slots_dev, const float* angles_dev, int num_positions, int rows, int q_heads,
                                int kv_heads, int head_dim, void* cache, int num_pages, int page_size, void* stream);
 
+/* Attention of the new tokens over the paged 4-bit cache. Request b's new tokens are rows row_starts[b] .. of q and
+ * out, new_lens[b] of them (at most max_new are served; row_starts and new_lens as df_page_plan leaves them, or both
+ * NULL: one row a request, row b); row j of them attends keys 0 .. seq_lens[b] - new_lens[b] + j, query head h reads
+ * key/value head h / (q_heads / kv_heads). Keys whose page is missing (page_table outside [0, num_pages)) do not count;
+ * a row without keys is zeros. Rows of no request are left as they were. `workspace`: device scratch of
+ * df_attention_paged4_workspace_bytes(), contents arbitrary, one for launches that can overlap. max_ctas limits the
+ * launch to that many SMs (0: all). Reproducible bit for bit at a given max_ctas. */
+size_t df_attention_paged4_workspace_bytes(int requests, int q_heads, int kv_heads, int max_new);
+int df_attention_paged4_bf16(const void* q, long long ld_q, const void* cache, const int* page_table_dev,
+                             const int* seq_lens_dev, const int* row_starts_dev, const int* new_lens_dev, void* out,
+                             long long ld_out, int rows, int requests, int max_pages, int num_pages, int page_size,
+                             int q_heads, int kv_heads, int head_dim, int max_new, float scale, void* workspace,
+                             size_t workspace_bytes, int max_ctas, df_status_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -117,3 +117,19 @@ def token_logprobs(logits: torch.Tensor, ids, top_k: int):
         tid.append(torch.tensor(order, dtype=torch.int32))
         tlp.append(logp[torch.tensor(order, dtype=torch.long)] if order else torch.zeros(0, dtype=torch.float64))
     return torch.stack(lp), torch.stack(ent), torch.stack(tid), torch.stack(tlp)
+
+
+def pack_granules(keys: torch.Tensor, values: torch.Tensor):
+    """``keys, values [16 n, 128]`` (bf16 values) -> the bytes ``uint8 [n, 2176]`` and the numbers (64 bits) they stand for."""
+    halves, stands = [], []
+    for x in (keys, values):
+        codes, scale, low = quantise(x)
+        b = (codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8).view(-1, GRANULE, 4, 16)
+        placed = torch.empty_like(b)
+        for r in range(GRANULE):
+            for c in range(4):
+                placed[:, r, c ^ ((r >> 1) & 3)] = b[:, r, c]
+        params = torch.cat([scale, low], 1).bfloat16().view(torch.uint8).view(-1, GRANULE * 4)
+        halves.append(torch.cat([placed.flatten(1), params], 1))
+        stands.append(scale * codes + low)
+    return torch.cat(halves, 1), stands[0], stands[1]

@@ -55,6 +55,59 @@ def test_append_refusals(native_lib):
     _refused(native_lib, -3, "2^31", "df_rope_append_paged4_bf16", *append(pages=1 << 28))
 
 
+def test_attention_refusals(native_lib):
+    keep, p = _buffer()
+    name = "df_attention_paged4_bf16"
+
+    def call(q=p, ld_q=512, starts=None, fresh=None, rows=2, requests=2, max_pages=4, page=16, hq=4, hkv=1, hd=128, max_new=1, scale=0.1, ws=p, ws_bytes=1 << 40):
+        return (q, ld_q, p, p, p, starts, fresh, p, 512, rows, requests, max_pages, 8, page, hq, hkv, hd, max_new, scale, ws, ws_bytes, 0, p, None)
+
+    _refused(native_lib, -1, "NULL", name, *call(ws=None))
+    _refused(native_lib, -1, "together", name, *call(starts=p))
+    _refused(native_lib, -1, "one row", name, *call(max_new=2))
+    _refused(native_lib, -1, "one row", name, *call(rows=1))
+    _refused(native_lib, -3, "head_dim", name, *call(hd=64))
+    _refused(native_lib, -1, "multiple of kv_heads", name, *call(hq=3, hkv=2))
+    _refused(native_lib, -1, "multiple of 16", name, *call(page=40))
+    _refused(native_lib, -3, "2^31", name, *call(max_pages=1 << 28))
+    _refused(native_lib, -3, "2^31", name, *call(starts=p, fresh=p, max_new=1 << 20, max_pages=1 << 20, hq=16, ld_q=2048))
+    _refused(native_lib, -1, "strides", name, *call(ld_q=504))
+    _refused(native_lib, -1, "aligned", name, *call(q=p + 8))
+    _refused(native_lib, -1, "scale", name, *call(scale=0.0))
+    _refused(native_lib, -1, "too small", name, *call(ws_bytes=1024))
+    assert native_lib.df_attention_paged4_workspace_bytes(0, 4, 1, 1) == 0
+    assert native_lib.df_attention_paged4_workspace_bytes(3, 4, 3, 1) == 0
+    # the scratch does not grow with the cache
+    assert 0 < native_lib.df_attention_paged4_workspace_bytes(256, 32, 8, 1) < 32 << 20
+
+
+def test_attention_wrapper_refuses_wrong_tensors():
+    from dynaflow_b200 import ops
+
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
+    q, cache = torch.zeros(2, 512, dtype=torch.bfloat16), ops.paged4_cache(4, 1, 16, device="cpu")
+    ws = torch.zeros(64, dtype=torch.uint8)
+    call = lambda q=q, cache=cache, table=i32(2, 3), lens=i32(2), out=q, ws=ws, **kw: ops.attention_paged4(q, cache, table, lens, out, ws, page_size=16, **kw)  # noqa: E731
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        call()
+    with pytest.raises(ValueError, match="bf16"):
+        call(q=q.float())
+    with pytest.raises(ValueError, match="Hq"):
+        call(out=torch.zeros(2, 256, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="seq_lens"):
+        call(lens=i32(3))
+    with pytest.raises(ValueError, match="together"):
+        call(new_lens=i32(2))
+    with pytest.raises(ValueError, match="row_starts"):
+        call(new_lens=i32(2), row_starts=i32(2))
+    with pytest.raises(ValueError, match="max_new must be 1"):
+        call(max_new=2)
+    with pytest.raises(ValueError, match="uint8"):
+        call(ws=ws.float())
+    with pytest.raises(ValueError, match="positive"):
+        ops.attention_paged4_workspace(2, 3, 2, device="cpu")
+
+
 def test_wrappers_refuse_wrong_tensors():
     from dynaflow_b200 import ops
 
