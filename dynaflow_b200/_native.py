@@ -98,6 +98,11 @@ SIGNATURES: dict[str, tuple] = {
     "df_attention_paged4_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "df_attention_paged4_bf16": (_i, [_vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
                                       _sz, _i, _vp, _vp]),
+    "df_token_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
+    "df_token_logprobs": (_i, [_vp, _i, _ll, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "df_token_logprobs_record_bytes": (_sz, [_i, _i]),
+    "df_token_logprobs_shard": (_i, [_vp, _i, _ll, _vp, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
+    "df_token_logprobs_join": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "df_mlp_gated_bf16_static": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

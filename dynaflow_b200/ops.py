@@ -494,3 +494,103 @@ def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
             hd ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), max_ctas,
             status_block(q.device).data_ptr(), _stream_ptr(q))
     return out
+
+
+# ------------------------------------------------------------ token log probabilities
+MAX_TOP_TOKENS = 32
+
+
+def token_logprobs_out(rows: int, top: int, device: torch.device | str = "cuda") -> tuple[torch.Tensor, ...]:
+    """Result tensors of ``token_logprobs``: log probabilities and entropies ``[rows]`` fp32, the most likely tokens' ids
+    (int32) and log probabilities (fp32) ``[rows, top]``."""
+    return (torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
+            torch.empty(rows, top, dtype=torch.int32, device=device), torch.empty(rows, top, dtype=torch.float32, device=device))
+
+
+def token_logprobs_workspace(rows: int, vocab: int, top: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """Scratch for ``token_logprobs`` / ``token_logprobs_shard``; its contents are arbitrary. Calls that can overlap on the
+    GPU, captured graphs included, need one each."""
+    need = int(_native.load().df_token_logprobs_workspace_bytes(rows, vocab, top))
+    if need == 0:
+        raise ValueError(f"rows and vocab must be positive, top 0 to {MAX_TOP_TOKENS}")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _require_logits(logits: torch.Tensor, ids: torch.Tensor) -> tuple[int, int]:
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
+        raise ValueError(f"logits must be 2-D bf16 or fp32 with unit inner stride, got {logits.dtype} {tuple(logits.shape)} "
+                         f"strides {logits.stride()}")
+    rows, vocab = logits.shape
+    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (rows,) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 or int64 tensor of {rows} entries, got {ids.dtype} {tuple(ids.shape)}")
+    return rows, vocab
+
+
+def _require_logprobs_out(out: tuple[torch.Tensor, ...], rows: int, top: int) -> None:
+    lp, ent, tid, tlp = out
+    for name, t, dtype, shape in (("logprob", lp, torch.float32, (rows,)), ("entropy", ent, torch.float32, (rows,)),
+                                  ("top_ids", tid, torch.int32, (rows, top)), ("top_logprobs", tlp, torch.float32, (rows, top))):
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out: tuple[torch.Tensor, ...] | None = None,
+                   workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
+    """``(logprob, entropy, top_ids, top_logprobs)`` of ``logits [rows, vocab]`` (bf16 or fp32, any row stride): the log
+    probability of ``ids [rows]``, the entropy (nats), and the ``top`` most likely tokens, largest first, of equal logits the
+    lower index first. Forbidden tokens are ``-inf``; a row of nothing else has log probabilities ``-inf`` and entropy 0."""
+    rows, vocab = _require_logits(logits, ids)
+    if out is None:
+        out = token_logprobs_out(rows, top, logits.device)
+    else:
+        _require_logprobs_out(out, rows, top)
+    if workspace is None and rows > 0:
+        workspace = token_logprobs_workspace(rows, vocab, top, logits.device)
+    idx = _same_device(logits, ids, workspace, *out)
+    if rows == 0:
+        return out
+    lp, ent, tid, tlp = out
+    _launch(idx, "df_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
+            ids.element_size(), rows, vocab, top, lp.data_ptr(), ent.data_ptr(), tid.data_ptr(), tlp.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(logits))
+    return out
+
+
+def token_logprobs_record(rows: int, top: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """One rank's record of ``rows`` rows (``token_logprobs_shard`` fills it)."""
+    need = int(_native.load().df_token_logprobs_record_bytes(rows, top))
+    if need == 0:
+        raise ValueError(f"rows must be positive, top 0 to {MAX_TOP_TOKENS}")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def token_logprobs_shard(logits: torch.Tensor, ids: torch.Tensor, vocab_start: int, top: int, record: torch.Tensor,
+                         workspace: torch.Tensor) -> torch.Tensor:
+    """This rank's part of ``token_logprobs`` when ``logits`` are tokens ``vocab_start ...`` of a split vocabulary (``ids`` are of
+    the whole one). The ranks' records, all-gathered in rank order, give the results with ``token_logprobs_join``."""
+    rows, vocab = _require_logits(logits, ids)
+    if record.dtype != torch.uint8 or not record.is_contiguous() or record.numel() < int(_native.load().df_token_logprobs_record_bytes(rows, top)):
+        raise ValueError("record must be a contiguous uint8 tensor from token_logprobs_record")
+    idx = _same_device(logits, ids, record, workspace)
+    if rows == 0:
+        return record
+    _launch(idx, "df_token_logprobs_shard", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
+            ids.element_size(), rows, vocab, vocab_start, top, record.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream_ptr(logits))
+    return record
+
+
+def token_logprobs_join(records: torch.Tensor, parts: int, rows: int, top: int, *, out: tuple[torch.Tensor, ...] | None = None) -> tuple[torch.Tensor, ...]:
+    """The results from the ``parts`` ranks' records, one behind the other."""
+    each = int(_native.load().df_token_logprobs_record_bytes(rows, top))
+    if each == 0 or records.dtype != torch.uint8 or not records.is_contiguous() or records.numel() != parts * each:
+        raise ValueError("records must be a contiguous uint8 tensor of the ranks' records")
+    if out is None:
+        out = token_logprobs_out(rows, top, records.device)
+    else:
+        _require_logprobs_out(out, rows, top)
+    idx = _same_device(records, *out)
+    lp, ent, tid, tlp = out
+    _launch(idx, "df_token_logprobs_join", records.data_ptr(), parts, rows, top, lp.data_ptr(), ent.data_ptr(), tid.data_ptr(),
+            tlp.data_ptr(), _stream_ptr(records))
+    return out

@@ -520,6 +520,28 @@ int df_attention_paged4_bf16(const void* q, long long ld_q, const void* cache, c
                              int q_heads, int kv_heads, int head_dim, int max_new, float scale, void* workspace,
                              size_t workspace_bytes, int max_ctas, df_status_t* dev_status, void* stream);
 
+/* ------------------------------------------------------- token log probabilities
+ *
+ * Of rows of logits (bf16, or fp32 with fp32 = 1; any row stride ld >= vocab in elements): the log probability of the
+ * row's given token (ids: int32 or int64 by id_bytes; an id outside the vocabulary gives -inf), the entropy in nats, and
+ * the `top` (0 to 32) most likely tokens with their log probabilities, largest first, of equal logits the lower index
+ * first. One pass over the logits; sums in fp32. Forbidden tokens are -inf; a row of nothing else has log probabilities
+ * -inf and entropy 0; a row with a NaN or +inf gives NaN. `workspace` (df_token_logprobs_workspace_bytes, contents
+ * arbitrary, one for launches that can overlap) holds the slices of rows. Deterministic. */
+size_t df_token_logprobs_workspace_bytes(int rows, int vocab, int top);
+int df_token_logprobs(const void* logits, int fp32, long long ld, const void* ids_dev, int id_bytes, int rows, int vocab,
+                      int top, float* logprob_dev, float* entropy_dev, int* top_ids_dev, float* top_logprobs_dev,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for a vocabulary whose logits are split over ranks: _shard writes this rank's record of every row
+ * (df_token_logprobs_record_bytes; its logits are tokens vocab_start ..., ids are of the whole vocabulary, top is at most
+ * the shard's size); the ranks' records one behind the other (all-gathered, in rank order) give the results with _join. */
+size_t df_token_logprobs_record_bytes(int rows, int top);
+int df_token_logprobs_shard(const void* logits, int fp32, long long ld, const void* ids_dev, int id_bytes, int rows, int vocab,
+                            int vocab_start, int top, void* record_dev, void* workspace, size_t workspace_bytes, void* stream);
+int df_token_logprobs_join(const void* records_dev, int parts, int rows, int top, float* logprob_dev, float* entropy_dev,
+                           int* top_ids_dev, float* top_logprobs_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

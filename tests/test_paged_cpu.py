@@ -154,3 +154,53 @@ def test_oracle_cache_round_trip():
         for got, want in ((k, x[i]), (v, y[i])):
             step = (want.max() - want.min()).double() / 15
             assert ((got - want.double()).abs() <= step * (0.5 + 15 * 2 ** -8)).all()     # the bf16 scale: 15 steps off by 2^-8 of one
+
+
+def test_logprob_refusals(native_lib):
+    keep, p = _buffer()
+    name = "df_token_logprobs"
+
+    def call(logits=p, fp32=0, ld=100, id_bytes=8, rows=2, vocab=100, top=5, lp=p, tid=p, ws=p, ws_bytes=1 << 30):
+        return (logits, fp32, ld, p, id_bytes, rows, vocab, top, lp, p, tid, p, ws, ws_bytes, None)
+
+    _refused(native_lib, -1, "NULL", name, *call(logits=None))
+    _refused(native_lib, -1, "NULL", name, *call(lp=None))
+    _refused(native_lib, -1, "NULL", name, *call(tid=None))
+    _refused(native_lib, -1, "positive", name, *call(rows=0))
+    _refused(native_lib, -1, "fp32", name, *call(fp32=2))
+    _refused(native_lib, -1, "4- or 8-byte", name, *call(id_bytes=2))
+    _refused(native_lib, -1, "stride", name, *call(ld=99))
+    _refused(native_lib, -3, "32", name, *call(top=33))
+    _refused(native_lib, -3, "vocabulary", name, *call(vocab=4, top=5))
+    _refused(native_lib, -1, "aligned", name, *call(logits=p + 1))
+    _refused(native_lib, -1, "too small", name, *call(vocab=100000, ld=100000, ws_bytes=8))
+    shard = "df_token_logprobs_shard"
+    _refused(native_lib, -1, "vocab_start", shard, p, 0, 100, p, 8, 2, 100, -1, 5, p, p, 1 << 30, None)
+    _refused(native_lib, -1, "NULL", shard, p, 0, 100, p, 8, 2, 100, 0, 5, None, p, 1 << 30, None)
+    join = "df_token_logprobs_join"
+    _refused(native_lib, -1, "parts", join, p, 65, 2, 5, p, p, p, p, None)
+    _refused(native_lib, -3, "top", join, p, 2, 2, 40, p, p, p, p, None)
+    assert native_lib.df_token_logprobs_workspace_bytes(0, 10, 0) == 0
+    assert native_lib.df_token_logprobs_record_bytes(3, 4) == 3 * (16 + 4 * 8)
+
+
+def test_logprob_wrappers_refuse_wrong_tensors():
+    from dynaflow_b200 import ops
+
+    x, ids = torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.token_logprobs(x, ids, 2)
+    with pytest.raises(ValueError, match="bf16 or fp32"):
+        ops.token_logprobs(x.half(), ids, 2)
+    with pytest.raises(ValueError, match="bf16 or fp32"):
+        ops.token_logprobs(x.T, ids, 2)
+    with pytest.raises(ValueError, match="ids"):
+        ops.token_logprobs(x, ids[:1], 2)
+    with pytest.raises(ValueError, match="top"):
+        ops.token_logprobs(x, ids, 33)
+    with pytest.raises(ValueError, match="top_ids"):
+        ops.token_logprobs(x, ids, 2, out=ops.token_logprobs_out(2, 3, "cpu"))
+    with pytest.raises(ValueError, match="record"):
+        ops.token_logprobs_shard(x, ids, 0, 2, torch.zeros(8, dtype=torch.uint8), torch.zeros(8, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="records"):
+        ops.token_logprobs_join(torch.zeros(8, dtype=torch.uint8), 2, 2, 2)
