@@ -23,11 +23,15 @@
 // what the tensor pipe would do in the time the bytes take, so it stays on the warp-level instructions: operands
 // come from registers, where the codes are unpacked, instead of going through shared or tensor memory again.)
 //
-// Work: the granules (16 tokens of a head) of all requests and heads in one list, cut evenly over all warps of
-// the launch, whatever the lengths. A warp walks its part on its own: its lanes issue the copies of its ring
-// (one contiguous 2176-byte bulk copy a granule), it keeps its own maximum, sum and O^T and never waits for
-// another warp. A request and head that lies inside one warp's part is written to the output at once; one that
-// is cut leaves a partial result a warp (at most two a warp), which a second launch merges in order.
+// Work: the tiles (32 tokens of a head, two granules) of all requests and heads in one list, cut evenly over the CTAs
+// and, inside a CTA, over its warps, whatever the lengths. A warp walks its part on its own: its lanes issue the copies
+// of its ring (one contiguous bulk copy a tile, two where a page ends inside it), it keeps its own reference, sums and
+// O^T and waits for no other warp. A request and head that lies inside one warp's part is written to the output at
+// once; one that is cut between warps is joined in shared memory at the end of the CTA; one that is cut between CTAs
+// leaves a partial result each (at most two a CTA), and the CTA that finishes last joins them in the order of the CTAs
+// (a counter a cut, which that CTA sets back to zero).
+// A request and head costs a warp its queries and its result as well as its tiles, so it counts SEGMENT_COST tiles
+// more when the list is cut (without: 16 requests of a few tokens among long ones make one CTA twice as long).
 //
 // Bound: HBM, 136 bytes a key and head.
 #include <cuda_bf16.h>
@@ -42,9 +46,13 @@ namespace df {
 namespace paged {
 
 constexpr int WHERE_PAGED_ATTN = 51;
-constexpr int ATTN_MIN_PART = 2;       // granules a warp takes at least
-constexpr float RESCALE_LIMIT = 8.0f;  // the reference maximum moves when a score exceeds it by 2^8
-constexpr int PARTIAL_FLOATS = HEAD_DIM + 2;
+constexpr float RESCALE_LIMIT = 8.0f;         // the reference moves when a score exceeds it by 2^8
+constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padded to 16 bytes
+constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
+constexpr int TILE = 2 * GRANULE;             // tokens
+constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
+constexpr unsigned SEGMENT_COST = 2;          // tiles
+constexpr int MAX_COLUMNS = 1 << 20;
 
 struct AttnParams {
   const __nv_bfloat16* q;
@@ -54,40 +62,53 @@ struct AttnParams {
   const int* row_starts;  // may be null: request b is row b
   const int* new_lens;    // may be null: one row a request
   __nv_bfloat16* out;
-  float* partial;         // [workers][2][columns][PARTIAL_FLOATS]
-  long long* prefix;      // [requests + 1] granules before a request
+  float* partial;         // [ctas][2][columns][PARTIAL_FLOATS]
+  int* arrived;           // [ctas] CTAs that have left their part of the request and head whose first part is CTA c's; zero between launches
+  uint2* prefix;          // [requests] what lies before a request: tiles, segments
   long long ld_q, ld_out;
   int rows, requests, max_pages, num_pages, page_granules;
   int q_heads, kv_heads, group, max_new;
-  float scale_log2;
+  float scale_log2, inv_group;
   unsigned long long timeout_ns;
   Status* status;
 };
 
-// What a request adds to the list of granules.
+// x / d of small whole numbers (below 2^20) by the reciprocal of d.
+__device__ __forceinline__ int div_small(int x, float inv) { return static_cast<int>((static_cast<float>(x) + 0.5f) * inv); }
+
+// What a request adds to the list: segments (a key/value head and set of columns) of `tiles` each.
 struct Weight {
-  int len, fresh, granules, blocks;  // blocks: sets of columns (new token x head of the group) of a key/value head
-  __device__ __forceinline__ int total(int kv_heads) const { return granules * blocks * kv_heads; }
+  int len, fresh, tiles, blocks;  // blocks: sets of columns (new token x head of the group) of a key/value head
 };
 
 template <int COLS>
-__device__ __forceinline__ Weight request_weight(const AttnParams& p, int b) {
+__device__ __forceinline__ Weight weight_of(const AttnParams& p, int len, int fresh) {
   Weight w;
-  w.len = static_cast<int>(min(static_cast<long long>(max(p.seq_lens[b], 0)), static_cast<long long>(p.max_pages) * p.page_granules * GRANULE));
-  w.fresh = p.new_lens != nullptr ? p.new_lens[b] : 1;
-  const int served = min(w.fresh, p.max_new);
-  w.granules = max((w.len + GRANULE - 1) / GRANULE, 1);  // a row without keys still has its output (zeros) to be written
+  w.len = len;
+  w.fresh = fresh;
+  const int served = min(fresh, p.max_new);
+  w.tiles = max((len + TILE - 1) / TILE, 1);  // a row without keys still has its output (zeros) to be written
   w.blocks = served > 0 ? (served * p.group + COLS - 1) / COLS : 0;
   return w;
 }
-
-// Worker w of `workers` takes granules [part_start(w), part_start(w + 1)).
-__device__ __forceinline__ long long part_start(long long total, long long workers, long long w) { return total * w / workers; }
-__device__ __forceinline__ long long part_of(long long total, long long workers, long long f) { return ((f + 1) * workers - 1) / total; }
-__device__ __forceinline__ long long worker_count(long long total, long long most) {
-  const long long n = total / ATTN_MIN_PART;
-  return n < 1 ? 1 : (n < most ? n : most);
+template <int COLS>
+__device__ __forceinline__ Weight load_weight(const AttnParams& p, int b) {
+  const int len = static_cast<int>(min(static_cast<long long>(max(p.seq_lens[b], 0)), static_cast<long long>(p.max_pages) * p.page_granules * GRANULE));
+  return weight_of<COLS>(p, len, p.new_lens != nullptr ? p.new_lens[b] : 1);
 }
+
+// The list is cut by cost (tiles and SEGMENT_COST a segment) into parts that differ by one at most. A CTA has work
+// for every warp before there is another one.
+struct Cut {
+  unsigned parts, each, longer;  // the first `longer` parts are each + 1 long, the others each
+  __device__ __forceinline__ Cut(unsigned cost, unsigned n) : parts(n), each(cost / n), longer(cost - each * n) {}
+  __device__ __forceinline__ unsigned start(unsigned c) const { return each * c + min(c, longer); }
+  __device__ __forceinline__ unsigned part_of(unsigned at) const {
+    const unsigned head = longer * (each + 1);
+    return at < head ? at / (each + 1) : longer + (at - head) / each;
+  }
+};
+__device__ __forceinline__ unsigned cost_of(const uint2& v) { return v.x + SEGMENT_COST * v.y; }
 
 __device__ __forceinline__ float ex2f(float x) {
   float r;
@@ -110,13 +131,18 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Two pairs of codes of a 32-bit word as fp16 subnormals: n 2^-24 and 16 n 2^-24.
 __device__ __forceinline__ uint32_t code_lo(uint32_t w) { return w & 0x000f000fu; }
@@ -133,22 +159,89 @@ __device__ __forceinline__ float max_rows(float v) {
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
+// A tile in the ring. `flags`: tile of the segment << 3, whether its segment's first tile of this part, whether each
+// of its granules has a page.
 struct Desc {
-  int b, hc, g, page_ok;  // request, key/value head * blocks + block, granule of the request, whether its page exists
+  int flags, b, hc;  // request, key/value head * blocks + block
+};
+constexpr int TILE_FIRST = 4, TILE_PAGES = 3;
+
+// What a warp leaves of requests it does not hold whole: `head` began in an earlier warp, `tail` goes on in a later one.
+struct Ends {
+  int head_b, head_hc, head_ends;  // head_b < 0: none; head_ends: its last tile is in this warp
+  int tail_b, tail_hc;             // tail_b < 0: none
+  int used;                        // whether the warp has tiles
 };
 
 template <int NT, int WARPS, int STAGES>
 struct AttnShared {
-  uint8_t ring[WARPS][STAGES][GRANULE_BYTES];
+  static constexpr int COLS = 8 * NT;
+  uint8_t ring[WARPS][STAGES][TILE_BYTES];       // at the end a warp's tail lies in its own ring
+  float head[WARPS][COLS][PARTIAL_FLOATS];
   Desc desc[WARPS][STAGES];
   uint64_t full[WARPS][STAGES];
+  uint2 prefix[REQUESTS_IN_SMEM];
+  int2 lens[REQUESTS_IN_SMEM];                   // length, new tokens
+  uint2 warp_sum[WARPS];
+  Ends ends[WARPS];
+  int order[WARPS];                              // the warps that have tiles
   uint32_t abort;
+  int joins[2];                                  // whether this CTA joins the parts of its first / last segment
+  static_assert(STAGES * TILE_BYTES >= COLS * PARTIAL_FLOATS * 4, "the tail fits into the ring");
 };
+
+// Weighted sum of one column of the partial results `link(i)`, i in [0, n): lane l has dimensions 4l .. 4l + 3.
+// Results are relative to the largest reference; `sum` and `ref` are the joined ones. Eight parts are in flight at a time.
+template <typename Link>
+__device__ __forceinline__ float4 join_links(int n, Link link, int lane, float& sum, float& ref) {
+  float best = -INFINITY;
+  sum = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float4 v[8];
+    float2 ml[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < n) {
+        const float* s = link(i0 + i);
+        v[i] = *reinterpret_cast<const float4*>(s + 4 * lane);
+        ml[i] = *reinterpret_cast<const float2*>(s + HEAD_DIM);
+      } else {
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ml[i] = make_float2(0.f, 0.f);
+      }
+    float top = best;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = ml[i].y != 0.0f ? fmaxf(top, ml[i].x) : top;  // a part without keys has no reference
+    const float keep = best == -INFINITY ? 0.0f : ex2f(best - top);
+    best = top;
+    sum *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = ml[i].y == 0.0f ? 0.0f : ex2f(ml[i].x - top);
+      sum = fmaf(f, ml[i].y, sum);
+      acc.x = fmaf(f, v[i].x, acc.x);
+      acc.y = fmaf(f, v[i].y, acc.y);
+      acc.z = fmaf(f, v[i].z, acc.z);
+      acc.w = fmaf(f, v[i].w, acc.w);
+    }
+  }
+  ref = best == -INFINITY ? 0.0f : best;
+  return acc;
+}
+__device__ __forceinline__ void store_row(__nv_bfloat16* dst, float4 v, float sum) {
+  const bool any = sum != 0.0f;  // no keys: zeros
+  const float inv = 1.0f / sum;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? v.x * inv : 0.f, any ? v.y * inv : 0.f);
+  const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? v.z * inv : 0.f, any ? v.w * inv : 0.f);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
 
 // NT: sets of 8 columns a warp carries. One CTA an SM; the registers of a warp decide how many warps it has.
 template <int NT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const AttnParams p) {
-  constexpr int COLS = 8 * NT;
+  constexpr int COLS = 8 * NT, THREADS = WARPS * 32;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<AttnShared<NT, WARPS, STAGES>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -156,96 +249,119 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   if (lane < STAGES) mbar_init(&sm.full[warp][lane], 1);
   if (threadIdx.x == 0) sm.abort = 0u;
   mbar_fence_init();
-  __syncthreads();
   const Deadline dl{globaltimer_ns() + p.timeout_ns, &sm.abort, p.status};
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // ---- the whole list, and this warp's part of it
-  long long total = 0;
-  for (int b0 = 0; b0 < p.requests; b0 += 32) {
-    const int b = b0 + lane;
-    long long w = b < p.requests ? request_weight<COLS>(p, b).total(p.kv_heads) : 0;
-    if (blockIdx.x == 0 && warp == 0) {
-      long long inc = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      if (b < p.requests) p.prefix[b] = total + inc - w;
+  // ---- prefix sums over the requests (many requests: in the workspace, where every CTA writes the same numbers)
+  const bool in_smem = p.requests <= REQUESTS_IN_SMEM;
+  uint2* prefix = in_smem ? sm.prefix : p.prefix;
+  uint2 all{0, 0};
+  for (int b0 = 0; b0 < p.requests; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    uint2 v{0, 0};
+    if (b < p.requests) {
+      const Weight w = load_weight<COLS>(p, b);
+      v.y = static_cast<unsigned>(w.blocks) * p.kv_heads;
+      v.x = v.y * w.tiles;
+      if (in_smem) sm.lens[b] = make_int2(w.len, w.fresh);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    total += w;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.requests] = total;
-  if (total == 0) return;
-  const long long workers = worker_count(total, static_cast<long long>(gridDim.x) * WARPS);
-  const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;  // neighbours in the list are on different SMs
-  if (worker >= workers) return;
-  const long long f0 = part_start(total, workers, worker);
-  const int count = static_cast<int>(part_start(total, workers, worker + 1) - f0);
-
-  // first request of the part
-  int cur_b = 0;
-  long long rel0 = f0;
-  for (int b0 = 0;; b0 += 32) {
-    const int b = b0 + lane;
-    const long long w = b < p.requests ? request_weight<COLS>(p, b).total(p.kv_heads) : 0;
-    long long inc = w;
+    uint2 inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
+      const unsigned ux = __shfl_up_sync(0xffffffffu, inc.x, o), uy = __shfl_up_sync(0xffffffffu, inc.y, o);
+      if (lane >= o) {
+        inc.x += ux;
+        inc.y += uy;
+      }
     }
-    const unsigned past = __ballot_sync(0xffffffffu, inc > rel0);  // the request ends behind the start
-    if (past != 0u) {
-      const int src = __ffs(past) - 1;
-      cur_b = b0 + src;
-      rel0 -= __shfl_sync(0xffffffffu, inc - w, src);
-      break;
+    if (b0 > 0) __syncthreads();
+    if (lane == 31) sm.warp_sum[warp] = inc;
+    __syncthreads();
+    uint2 before = all;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      const uint2 s = sm.warp_sum[i];
+      if (i < warp) {
+        before.x += s.x;
+        before.y += s.y;
+      }
+      all.x += s.x;
+      all.y += s.y;
     }
-    rel0 -= __shfl_sync(0xffffffffu, inc, 31);
-    if (b0 + 32 >= p.requests) return;  // cannot be: the part lies inside the list
+    if (b < p.requests) prefix[b] = make_uint2(before.x + inc.x - v.x, before.y + inc.y - v.y);
   }
-  int cur_rel = static_cast<int>(rel0);
+  if (all.x == 0) return;
+  const unsigned cost = cost_of(all);
+  const Cut cut(cost, min(static_cast<unsigned>(gridDim.x), (cost + WARPS - 1) / WARPS));
+  if (blockIdx.x >= cut.parts) return;
+  if (threadIdx.x < 2) sm.joins[threadIdx.x] = 0;
+  __syncthreads();
 
-  // ---- copies: lane i looks up the i-th of the next 32 granules; `issue(n)` starts the copy of granule n of the part
-  Desc ahead{0, 0, 0, 0};
-  const uint8_t* ahead_src = nullptr;
-  auto look_up = [&](int n0) {
-    int b = cur_b, rel = cur_rel + lane;
-    Weight w = request_weight<COLS>(p, b);
-    int all = w.total(p.kv_heads);
-    while (rel >= all && b + 1 < p.requests) {
-      rel -= all;
-      w = request_weight<COLS>(p, ++b);
-      all = w.total(p.kv_heads);
+  auto weight = [&](int b) { return in_smem ? weight_of<COLS>(p, sm.lens[b].x, sm.lens[b].y) : load_weight<COLS>(p, b); };
+  // the last request for which `before` (of what lies before it) is at most x: it is not empty
+  auto find = [&](unsigned x, auto before) {
+    int lo = 0, hi = p.requests;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before(prefix[mid]) <= x) lo = mid; else hi = mid;
     }
-    cur_b = __shfl_sync(0xffffffffu, b, 31);
-    cur_rel = __shfl_sync(0xffffffffu, rel, 31) + 1;
-    ahead.page_ok = 0;
-    if (n0 + lane < count) {
+    return lo;
+  };
+  // tiles that lie before a place of the list given as cost
+  auto tiles_before = [&](unsigned at) {
+    if (at >= cost) return all.x;
+    const int b = find(at, [](const uint2& v) { return cost_of(v); });
+    const unsigned tiles = weight(b).tiles, rel = at - cost_of(prefix[b]), each = tiles + SEGMENT_COST;
+    const unsigned s = rel / each, in = rel - s * each;
+    return prefix[b].x + s * tiles + (in > SEGMENT_COST ? in - SEGMENT_COST : 0u);
+  };
+  // the parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins
+  const unsigned at0 = cut.start(blockIdx.x), at_n = cut.start(blockIdx.x + 1) - at0;
+  const unsigned cut_at = tiles_before(at0 + Cut(at_n, WARPS).start(min(lane, WARPS)));
+  const unsigned f0 = __shfl_sync(0xffffffffu, cut_at, warp);
+  const int count = static_cast<int>(__shfl_sync(0xffffffffu, cut_at, warp + 1) - f0);
+
+  // ---- copies: lane i looks up the i-th of the next 32 tiles; `issue(s)` starts the copies of its tile into stage s
+  Desc ahead{0, 0, 0};
+  const uint8_t* ahead_src[2] = {nullptr, nullptr};
+  auto look_up = [&](int n) {
+    if (n + lane < count) {
+      const unsigned f = f0 + n + lane;
+      const int b = find(f, [](const uint2& v) { return v.x; });
+      const Weight w = weight(b);
+      const unsigned rel = f - prefix[b].x, hc = rel / w.tiles;
+      const int tile = static_cast<int>(rel - hc * w.tiles);
       ahead.b = b;
-      ahead.hc = rel / w.granules;
-      ahead.g = rel - ahead.hc * w.granules;
-      const int column = ahead.g / p.page_granules;
-      const int page = column < p.max_pages && w.len > 0 ? p.table[static_cast<size_t>(b) * p.max_pages + column] : -1;
-      if (page >= 0 && page < p.num_pages) {
-        ahead.page_ok = 1;
-        ahead_src = p.cache + ((static_cast<size_t>(page) * p.kv_heads + ahead.hc / w.blocks) * p.page_granules + (ahead.g - column * p.page_granules)) * GRANULE_BYTES;
+      ahead.hc = static_cast<int>(hc);
+      ahead.flags = tile << 3 | (tile == 0 || n + lane == 0 ? TILE_FIRST : 0);
+      const int kvh = w.blocks == 1 ? ahead.hc : ahead.hc / w.blocks;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int granule = 2 * tile + h;
+        if (granule * GRANULE >= w.len) continue;
+        const int column = granule / p.page_granules;  // inside the table: the length is limited to what a row can hold
+        const int page = p.table[static_cast<size_t>(b) * p.max_pages + column];
+        if (page >= 0 && page < p.num_pages) {
+          ahead.flags |= 1 << h;
+          ahead_src[h] = p.cache + ((static_cast<size_t>(page) * p.kv_heads + kvh) * p.page_granules + (granule - column * p.page_granules)) * GRANULE_BYTES;
+        }
       }
     }
   };
-  auto issue = [&](int n) {  // by the lane that looked granule n up
-    const int s = n % STAGES;
+  auto issue = [&](int s) {  // by the lane that looked the tile up
     sm.desc[warp][s] = ahead;
-    if (ahead.page_ok) {
-      mbar_expect_tx(&sm.full[warp][s], GRANULE_BYTES);
-      bulk_load(sm.ring[warp][s], ahead_src, GRANULE_BYTES, &sm.full[warp][s]);
-    } else {
-      mbar_arrive(&sm.full[warp][s]);  // nothing to copy: its keys are masked
+    uint8_t* dst = sm.ring[warp][s];
+    uint64_t* bar = &sm.full[warp][s];
+    if ((ahead.flags & TILE_PAGES) == TILE_PAGES && ahead_src[1] == ahead_src[0] + GRANULE_BYTES) {
+      mbar_expect_tx(bar, TILE_BYTES);
+      bulk_load(dst, ahead_src[0], TILE_BYTES, bar);
+    } else {  // a page ends in the middle, or what is not there is not copied: its keys are masked
+      const int halves = (ahead.flags & 1) + (ahead.flags >> 1 & 1);
+      if (halves == 0) mbar_arrive(bar);
+      else mbar_expect_tx(bar, halves * GRANULE_BYTES);
+      if ((ahead.flags & 1) != 0) bulk_load(dst, ahead_src[0], GRANULE_BYTES, bar);
+      if ((ahead.flags & 2) != 0) bulk_load(dst + GRANULE_BYTES, ahead_src[1], GRANULE_BYTES, bar);
     }
   };
   look_up(0);
@@ -254,78 +370,85 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
 
   // ---- state of the segment (one request, key/value head and set of columns)
   uint32_t qf[NT][16];                        // Q^T fragments: pair p of the 16 this thread's 32 dimensions make
-  float c1[NT][2], c2[NT][2];                 // score = acc * c1 * s_k + m_k * c2, of columns 2t and 2t + 1
+  float c1[NT][2], sq[NT][2];                 // score = (acc s_k + sq m_k) c1, of columns 2t and 2t + 1
   int limit[NT][2];                           // keys a column sees
-  float m[NT][2], l[NT][2], pm[NT][2];        // reference maximum (log2), sum p, sum p m_v (this thread's keys)
+  float ref[NT][2], over[NT][2];              // reference (log2); a score that exceeds it by `over` moves it (-inf: none yet)
+  float l[NT][2], pm[NT][2];                  // sum p and sum p m_v, of this thread's keys
   float acc[NT][8][4];
   float v_scale = 1.0f, v_limit = -1.0f;      // p s_v is held times v_scale = 2^-v_exp; scales above v_limit move it
   int v_exp = -100;
-  int seg_b = -1, seg_hc = -1, seg_first = 0, seg_last = 0, seg_granules = 0, min_limit = 0;
+  int seg_b = -1, seg_hc = 0, seg_first = 0, seg_last = 0, min_limit = 0;
+  Ends ends{-1, -1, 0, -1, -1, count > 0 ? 1 : 0};
 
-  auto begin = [&](const Desc& d) {
-    seg_b = d.b;
-    seg_hc = d.hc;
-    seg_first = d.g;
-    const Weight w = request_weight<COLS>(p, d.b);
-    seg_granules = w.granules;
-    const int kvh = d.hc / w.blocks, block = d.hc - kvh * w.blocks;
+  // head, first column and first row of a segment
+  auto place = [&](const Weight& w, int b, int hc, int& kvh, int& column0, int& row0) {
+    kvh = w.blocks == 1 ? hc : hc / w.blocks;
+    column0 = (hc - kvh * w.blocks) * COLS;
+    row0 = p.row_starts != nullptr ? p.row_starts[b] : b;
+  };
+
+  auto begin = [&](int b, int hc, int tile) {
+    seg_b = b;
+    seg_hc = hc;
+    seg_first = tile;
+    const Weight w = weight(b);
+    int kvh, column0, row0;
+    place(w, b, hc, kvh, column0, row0);
     const int served = min(w.fresh, p.max_new);
-    const int row0 = p.row_starts != nullptr ? p.row_starts[d.b] : d.b;
     min_limit = w.len;
     v_scale = 1.0f;
     v_limit = -1.0f;
     v_exp = -100;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int c = block * COLS + nt * 8 + g;  // this lane's column of the B fragments
-      const int j = c / p.group, row = row0 + j;
+      const int c = column0 + nt * 8 + g;  // this lane's column of the B fragments
+      const int j = div_small(c, p.inv_group), row = row0 + j;
       const bool here = j < served && row >= 0 && row < p.rows;
       uint4 raw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         raw[i] = here ? *reinterpret_cast<const uint4*>(p.q + row * p.ld_q + (kvh * p.group + c - j * p.group) * HEAD_DIM + t * 32 + i * 8)
                       : make_uint4(0u, 0u, 0u, 0u);
-      float x[32];
-      float sum = 0.f, big = 0.f;
+      float x[32], big = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float most = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           x[i * 8 + 2 * k] = __uint_as_float(w4[k] << 16);
           x[i * 8 + 2 * k + 1] = __uint_as_float(w4[k] & 0xffff0000u);
+          most = fmaxf(fmaxf(most, fabsf(x[i * 8 + 2 * k])), fabsf(x[i * 8 + 2 * k + 1]));
         }
+        big = fmaxf(big, most);
       }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        sum += x[i];
-        big = fmaxf(big, fabsf(x[i]));
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      const int e = max(min(exponent_of(big), 127), -100);
-      const float up = pow2i(14 - e);
+      const int e = max(min(exponent_of(big), 117), -100);
+      const float up[2] = {pow2i(14 - e), pow2i(10 - e)};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // word i of the 16 bytes, nibbles k and k + 4: dimensions 8i + k and 8i + k + 4 (odd k: 16 times the code)
-          const float f = (k & 1) ? up * 0.0625f : up;
-          const __half2 h = __floats2half2_rn(x[i * 8 + k] * f, x[i * 8 + k + 4] * f);
+          const __half2 h = __floats2half2_rn(x[i * 8 + k] * up[k & 1], x[i * 8 + k + 4] * up[k & 1]);
           qf[nt][i * 4 + k] = *reinterpret_cast<const uint32_t*>(&h);
         }
-      const float a = p.scale_log2 * pow2i(e + 10 > 127 ? 127 : e + 10);  // 2^24 of the codes, 2^(e - 14) of q
-      const float b2 = p.scale_log2 * sum;
+      // the sum of q: its product with codes that are all one
+      float one[4];
+      mma_f16_first(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[nt][0], qf[nt][1]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mma_f16(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[nt][2 * i], qf[nt][2 * i + 1]);
+      const float a = p.scale_log2 * pow2i(e + 10);  // 2^24 of the codes, 2^(e - 14) of q
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int cc = 2 * t + k;  // the columns of this thread's scores: held by lane group cc
         c1[nt][k] = __shfl_sync(0xffffffffu, a, cc * 4);
-        c2[nt][k] = __shfl_sync(0xffffffffu, b2, cc * 4);
-        const int jj = (block * COLS + nt * 8 + cc) / p.group;
+        sq[nt][k] = one[k];
+        const int jj = div_small(column0 + nt * 8 + cc, p.inv_group);
         limit[nt][k] = jj < served ? min(w.len - w.fresh + jj + 1, w.len) : w.len;  // a column without a query is computed and dropped
-        m[nt][k] = -INFINITY;
+        ref[nt][k] = 0.f;
+        over[nt][k] = -INFINITY;
         l[nt][k] = 0.f;
         pm[nt][k] = 0.f;
       }
@@ -340,43 +463,49 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   };
 
   auto flush = [&]() {
-    const Weight w = request_weight<COLS>(p, seg_b);
-    const int kvh = seg_hc / w.blocks, block = seg_hc - kvh * w.blocks;
+    const Weight w = weight(seg_b);
+    const bool began = seg_first == 0, ended = seg_last == w.tiles - 1;
+    int kvh, column0, row0;
+    place(w, seg_b, seg_hc, kvh, column0, row0);
     const int served = min(w.fresh, p.max_new);
-    const int row0 = p.row_starts != nullptr ? p.row_starts[seg_b] : seg_b;
-    const bool began = seg_first == 0, whole = began && seg_last == seg_granules - 1;
     const float back = 16777216.0f * pow2i(v_exp);  // 2^24 of the codes
-    float* slot = p.partial + (worker * 2 + (began ? 1 : 0)) * COLS * PARTIAL_FLOATS;
+    float* part = nullptr;
+    if (!began) {
+      part = sm.head[warp][0];
+      ends.head_b = seg_b;
+      ends.head_hc = seg_hc;
+      ends.head_ends = ended;
+    } else if (!ended) {  // the last segment of the part: every copy into the ring has been read
+      part = reinterpret_cast<float*>(sm.ring[warp][0]);
+      ends.tail_b = seg_b;
+      ends.tail_hc = seg_hc;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float sum = sum_rows(l[nt][k]), add = sum_rows(pm[nt][k]);
-        const int local = nt * 8 + 2 * t + k, c = block * COLS + local;
-        const int j = c / p.group, row = row0 + j;
-        const bool any = sum != 0.0f;  // no keys: zeros
-        const float inv = whole ? 1.0f / sum : 1.0f;
+        const int local = nt * 8 + 2 * t + k, c = column0 + local;
+        const int j = div_small(c, p.inv_group), row = row0 + j;
+        if (j >= served || row < 0 || row >= p.rows) continue;
+        const float inv = part != nullptr ? 1.0f : (sum != 0.0f ? 1.0f / sum : 0.0f);  // no keys: zeros
+        const float f0 = back * inv, f1 = f0 * 0.0625f, more = add * inv;
+        float* dst = part + local * PARTIAL_FLOATS;
+        __nv_bfloat16* out = p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
           // dimensions 32 c4 + 4 g .. + 3: rows g and g + 8 of m-tiles 2 c4 and 2 c4 + 1
-          const float o0 = (acc[nt][2 * c4][k] * back + add) * inv, o1 = (acc[nt][2 * c4][2 + k] * (back * 0.0625f) + add) * inv;
-          const float o2 = (acc[nt][2 * c4 + 1][k] * back + add) * inv, o3 = (acc[nt][2 * c4 + 1][2 + k] * (back * 0.0625f) + add) * inv;
+          const float o0 = fmaf(acc[nt][2 * c4][k], f0, more), o1 = fmaf(acc[nt][2 * c4][2 + k], f1, more);
+          const float o2 = fmaf(acc[nt][2 * c4 + 1][k], f0, more), o3 = fmaf(acc[nt][2 * c4 + 1][2 + k], f1, more);
           const int dim = 32 * c4 + 4 * g;
-          if (whole) {
-            if (j < served && row >= 0 && row < p.rows) {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? o0 : 0.f, any ? o1 : 0.f), hi = __floats2bfloat162_rn(any ? o2 : 0.f, any ? o3 : 0.f);
-              *reinterpret_cast<uint2*>(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + dim) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-            }
+          if (part == nullptr) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(o0, o1), hi = __floats2bfloat162_rn(o2, o3);
+            *reinterpret_cast<uint2*>(out + dim) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
           } else {
-            *reinterpret_cast<float2*>(slot + local * PARTIAL_FLOATS + dim) = make_float2(o0, o1);
-            *reinterpret_cast<float2*>(slot + local * PARTIAL_FLOATS + dim + 2) = make_float2(o2, o3);
+            *reinterpret_cast<float4*>(dst + dim) = make_float4(o0, o1, o2, o3);
           }
         }
-        if (!whole && g == 0) {
-          slot[local * PARTIAL_FLOATS + HEAD_DIM] = m[nt][k];
-          slot[local * PARTIAL_FLOATS + HEAD_DIM + 1] = sum;
-        }
+        if (part != nullptr && g == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = make_float2(ref[nt][k], sum);
       }
   };
 
@@ -386,80 +515,98 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   const uint32_t k_off = g * CODE_BYTES + (chunk_place(t, g) << 4);
 
   bool ok = true;
+  int stage = 0, phase = 0, base = 0;  // ring position of tile n; first tile of the last look-up
   for (int n = 0; n < count; ++n) {
-    const int s = n % STAGES;
-    ok = mbar_wait(&sm.full[warp][s], (n / STAGES) & 1, dl, WHERE_PAGED_ATTN, static_cast<unsigned>(worker));
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    const Desc d = sm.desc[warp][s];
-    if (d.b != seg_b || d.hc != seg_hc) {
-      if (seg_b >= 0) flush();
-      begin(d);
+    const int flags = sm.desc[warp][stage].flags, tile = flags >> 3;
+    if ((flags & TILE_FIRST) != 0) {
+      if (n > 0) flush();
+      begin(sm.desc[warp][stage].b, sm.desc[warp][stage].hc, tile);
     }
-    seg_last = d.g;
-    const uint8_t* st = sm.ring[warp][s];
-    const uint32_t st_addr = smem_u32(st);
-    const int key0 = d.g * GRANULE + g;  // this thread's keys: key0 and key0 + 8
-    const bool edge = d.page_ok == 0 || (d.g + 1) * GRANULE > min_limit;
+    seg_last = tile;
+    const bool there = mbar_try_wait(&sm.full[warp][stage], phase);
+    if (!__all_sync(0xffffffffu, there)) {
+      ok = mbar_wait(&sm.full[warp][stage], phase, dl, WHERE_PAGED_ATTN, blockIdx.x);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+    }
+    const uint8_t* st = sm.ring[warp][stage];
+    const bool edge = (flags & TILE_PAGES) != TILE_PAGES || (tile + 1) * TILE > min_limit;
 
     // ---- S^T = K Q^T
-    float sc[NT][4];
+    float sc[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) sc[nt][k] = 0.f;
-    {
-      const uint4 ka = *reinterpret_cast<const uint4*>(st + k_off), kb = *reinterpret_cast<const uint4*>(st + k_off + 8 * CODE_BYTES);
+    for (int h = 0; h < 2; ++h) {
+      const uint4 ka = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off), kb = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off + 8 * CODE_BYTES);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a8 = wa[i] >> 8, b8 = wb[i] >> 8;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_f16(sc[nt], code_lo(wa[i]), code_lo(wb[i]), code_hi(wa[i]), code_hi(wb[i]), qf[nt][4 * i], qf[nt][4 * i + 1]);
-          mma_f16(sc[nt], code_lo(a8), code_lo(b8), code_hi(a8), code_hi(b8), qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+          if (i == 0) mma_f16_first(sc[h][nt], code_lo(wa[i]), code_lo(wb[i]), code_hi(wa[i]), code_hi(wb[i]), qf[nt][4 * i], qf[nt][4 * i + 1]);
+          else mma_f16(sc[h][nt], code_lo(wa[i]), code_lo(wb[i]), code_hi(wa[i]), code_hi(wb[i]), qf[nt][4 * i], qf[nt][4 * i + 1]);
+          mma_f16(sc[h][nt], code_lo(a8), code_lo(b8), code_hi(a8), code_hi(b8), qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
         }
       }
     }
-    // ---- parameters of the two keys
-    float ks[2], km[2], vs[2], vm[2];
+    // ---- scores less their reference, log2
+    float vs[2][2], vm[2][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + PARAM_OFFSET + (g + 8 * r) * 4);
-      const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
-      ks[r] = __uint_as_float(kp << 16);
-      km[r] = __uint_as_float(kp & 0xffff0000u);
-      vs[r] = __uint_as_float(vp << 16);
-      vm[r] = __uint_as_float(vp & 0xffff0000u);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + PARAM_OFFSET + (g + 8 * r) * 4);
+        const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
+        const float ks = __uint_as_float(kp << 16), km = __uint_as_float(kp & 0xffff0000u);
+        vs[h][r] = __uint_as_float(vp << 16);
+        vm[h][r] = __uint_as_float(vp & 0xffff0000u);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& x = sc[h][nt][2 * r + c];
+            x = fmaf(fmaf(x, ks, sq[nt][c] * km), c1[nt][c], -ref[nt][c]);
+          }
+      }
+    bool careful = false;  // a key that only some columns see has parameters that are no numbers
+    if (edge) {            // masked keys: no score, and parameters (whatever lies there) that count for nothing
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const bool page = (flags >> h & 1) != 0;
+          const int key = tile * TILE + h * GRANULE + g + 8 * r;
+          bool any = false, every = true;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const bool seen = page && key < limit[nt][c];
+              any = any || seen;
+              every = every && seen;
+              if (!seen) sc[h][nt][2 * r + c] = -INFINITY;
+            }
+          if (!any) vs[h][r] = vm[h][r] = 0.f;
+          careful = careful || (any && !every && !(fabsf(vs[h][r]) + fabsf(vm[h][r]) < INFINITY));
+        }
+      careful = __any_sync(0xffffffffu, careful);
     }
-    bool seen[NT][4];
-    bool move = false;
+    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+    float top[NT][2];
+    bool move = vmax > v_limit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = k >> 1, c = k & 1;
-        sc[nt][k] = fmaf(sc[nt][k], c1[nt][c] * ks[r], c2[nt][c] * km[r]);
-        seen[nt][k] = true;
-        if (edge) {
-          seen[nt][k] = d.page_ok != 0 && key0 + 8 * r < limit[nt][c];
-          if (!seen[nt][k]) sc[nt][k] = -INFINITY;
-        }
-        move = move || sc[nt][k] > m[nt][c] + RESCALE_LIMIT;
+      for (int c = 0; c < 2; ++c) {
+        top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
+        move = move || top[nt][c] > over[nt][c];
       }
-    float vmax = 0.f;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      bool any = seen[0][2 * r] || seen[0][2 * r + 1];
-      if (NT == 2) any = any || seen[NT - 1][2 * r] || seen[NT - 1][2 * r + 1];
-      if (any) vmax = fmaxf(vmax, vs[r]);
-    }
-    move = move || vmax > v_limit;
     if (__any_sync(0xffffffffu, move)) {
       // new references: the largest score of each column so far, the power of two above the largest scale so far
+      float most = vmax;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-      const int e_new = max(v_exp, min(max(exponent_of(vmax) + 1, -100), 126));
+      for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const int e_new = max(v_exp, min(max(exponent_of(most) + 1, -100), 126));
       const float beta = e_new == v_exp ? 1.0f : pow2i(max(v_exp - e_new, -126));
       v_exp = e_new;
       v_scale = pow2i(-e_new);
@@ -468,9 +615,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float top = fmaxf(m[nt][c], max_rows(fmaxf(sc[nt][c], sc[nt][2 + c])));
-          const float alpha = top == -INFINITY ? 1.0f : ex2f(m[nt][c] - top);
-          m[nt][c] = top;
+          const bool none = over[nt][c] == -INFINITY;  // no key so far
+          const float high = max_rows(top[nt][c]), up = none ? high : fmaxf(high, 0.0f);
+          const float rise = up != -INFINITY ? up : 0.0f;
+          const float alpha = none ? 1.0f : ex2f(-rise);
+          if (up != -INFINITY) over[nt][c] = RESCALE_LIMIT;
+          ref[nt][c] += rise;
           l[nt][c] *= alpha;
           pm[nt][c] *= alpha;
           const float both = alpha * beta;
@@ -479,109 +629,172 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             acc[nt][i][c] *= both;
             acc[nt][i][2 + c] *= both;
           }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sc[h][nt][c] -= rise;
+            sc[h][nt][2 + c] -= rise;
+          }
         }
     }
-    // ---- P^T
-    uint32_t pf[NT][2];
-    const float vsn[2] = {vs[0] * v_scale, vs[1] * v_scale};
+    // ---- P^T, then O^T += V^T P^T
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
+    for (int h = 0; h < 2; ++h) {
+      uint32_t pf[NT][2];
+      const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * v_scale};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = k >> 1, c = k & 1;
-        const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-        const float e = ex2f(sc[nt][k] - ref);
-        l[nt][c] += e;
-        if (edge) {  // what lies at a masked key (also NaN parameters) counts for nothing
-          w[k] = seen[nt][k] ? e * vsn[r] : 0.f;
-          pm[nt][c] += seen[nt][k] ? e * vm[r] : 0.f;
-        } else {
-          w[k] = e * vsn[r];
-          pm[nt][c] = fmaf(e, vm[r], pm[nt][c]);
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = k >> 1, c = k & 1;
+          const float pr = ex2f(sc[h][nt][k]);
+          l[nt][c] += pr;
+          w[k] = pr * vsn[r];
+          if (!careful) pm[nt][c] = fmaf(pr, vm[h][r], pm[nt][c]);
         }
+        if (careful) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bool seen = sc[h][nt][k] != -INFINITY;
+            pm[nt][k & 1] += seen ? ex2f(sc[h][nt][k]) * vm[h][k >> 1] : 0.0f;
+            if (!seen) w[k] = 0.0f;
+          }
+        }
+        const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+        pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
+        pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
       }
-      const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
-      pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
-      pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
-    }
-    // ---- O^T += V^T P^T
+      const uint32_t st_addr = smem_u32(st) + h * GRANULE_BYTES;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t v[4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
-      ldmatrix_x4_trans(st_addr + (lm_off ^ (half * 32)), v);
+      for (int half = 0; half < 2; ++half) {
+        uint32_t v[4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
+        ldmatrix_x4_trans(st_addr + (lm_off ^ (half * 32)), v);
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        const uint32_t x0 = v[2 * cc], x1 = v[2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+        for (int cc = 0; cc < 2; ++cc) {
+          const uint32_t x0 = v[2 * cc], x1 = v[2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_f16(acc[nt][4 * half + 2 * cc], code_lo(x0), code_hi(x0), code_lo(x1), code_hi(x1), pf[nt][0], pf[nt][1]);
-          mma_f16(acc[nt][4 * half + 2 * cc + 1], code_lo(y0), code_hi(y0), code_lo(y1), code_hi(y1), pf[nt][0], pf[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(acc[nt][4 * half + 2 * cc], code_lo(x0), code_hi(x0), code_lo(x1), code_hi(x1), pf[nt][0], pf[nt][1]);
+            mma_f16(acc[nt][4 * half + 2 * cc + 1], code_lo(y0), code_hi(y0), code_lo(y1), code_hi(y1), pf[nt][0], pf[nt][1]);
+          }
         }
       }
     }
     __syncwarp();  // every lane has read the stage
     const int next = n + STAGES;
     if (next < count) {
-      if ((next & 31) == 0) look_up(next);
-      if (lane == (next & 31)) issue(next);
+      if (next - base == 32) look_up(base = next);
+      if (lane == next - base) issue(stage);
       __syncwarp();
+    }
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
     }
   }
   if (ok) {
-    flush();
+    __syncwarp();
+    if (count > 0) flush();
   } else {
     // a wait ran out: this warp's copies may still be on their way into shared memory
     const uint64_t t_stop = globaltimer_ns() + 2000000ull;
     while (globaltimer_ns() < t_stop) __nanosleep(1000);
   }
-}
+  if (lane == 0) sm.ends[warp] = ends;
+  __syncthreads();
 
-// Merges the partial results of requests and heads that were cut between warps, in the order of the warps:
-// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i. One warp a (request, new token, query head).
-template <int COLS>
-__global__ void attention_paged4_merge_kernel(const AttnParams p, int attn_ctas, int attn_warps) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const long long id = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (id >= static_cast<long long>(p.requests) * p.max_new * p.q_heads) return;
-  const int b = static_cast<int>(id / (p.max_new * p.q_heads));
-  const int rest = static_cast<int>(id - static_cast<long long>(b) * p.max_new * p.q_heads);
-  const int j = rest / p.q_heads, head = rest - j * p.q_heads;
-  const Weight w = request_weight<COLS>(p, b);
-  if (j >= min(w.fresh, p.max_new)) return;
-  const int row = (p.row_starts != nullptr ? p.row_starts[b] : b) + j;
-  if (row < 0 || row >= p.rows) return;
-  const int kvh = head / p.group, c = j * p.group + head - kvh * p.group;
-  const int block = c / COLS, local = c - block * COLS;
-  const long long total = p.prefix[p.requests];
-  const long long workers = worker_count(total, static_cast<long long>(attn_ctas) * attn_warps);
-  const long long first = p.prefix[b] + static_cast<long long>(kvh * w.blocks + block) * w.granules;
-  const long long w0 = part_of(total, workers, first), w1 = part_of(total, workers, first + w.granules - 1);
-  if (w0 == w1) return;  // written by the attention launch
-  float best = -INFINITY;
-  for (long long i = w0 + lane; i <= w1; i += 32)
-    best = fmaxf(best, p.partial[((i * 2 + (i == w0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS + HEAD_DIM]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-  float o4[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (long long i = w0; i <= w1; ++i) {
-    const float* s = p.partial + ((i * 2 + (i == w0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS;
-    const float f = s[HEAD_DIM] == -INFINITY ? 0.f : ex2f(s[HEAD_DIM] - best);
-    const float2 a = *reinterpret_cast<const float2*>(s + lane * 4), c2 = *reinterpret_cast<const float2*>(s + lane * 4 + 2);
-    sum += f * s[HEAD_DIM + 1];
-    o4[0] += f * a.x;
-    o4[1] += f * a.y;
-    o4[2] += f * c2.x;
-    o4[3] += f * c2.y;
+  // ---- what is cut between warps: a chain begins with a warp's tail (or with the first warp's head, which began in the
+  // CTA before) and goes through the heads of the following warps. One warp a chain and column.
+  const unsigned used = __ballot_sync(0xffffffffu, lane < WARPS && sm.ends[lane < WARPS ? lane : 0].used != 0);
+  const int active = __popc(used);
+  if (lane < WARPS && (used >> lane & 1u) != 0u) sm.order[__popc(used & ((1u << lane) - 1u))] = lane;  // every warp writes the same
+  __syncwarp();
+  if (active == 0) return;
+  const unsigned tails = __ballot_sync(0xffffffffu, lane < active && sm.ends[sm.order[lane < active ? lane : 0]].tail_b >= 0);
+  const int before = sm.ends[sm.order[0]].head_b >= 0 ? 1 : 0, chains = before + __popc(tails);
+  if (chains == 0) return;
+  struct Chain {
+    int b, hc, start, links;  // start: place among the warps with work of the one whose tail it begins with, -1: the first one's head
+    bool ended;
+  };
+  const unsigned ending = __ballot_sync(0xffffffffu, lane < active && sm.ends[sm.order[lane < active ? lane : 0]].head_ends != 0);
+  auto chain_of = [&](int k) {
+    Chain c;
+    unsigned later = tails;
+    for (int i = before; i < k; ++i) later &= later - 1u;
+    c.start = k < before ? -1 : __ffs(later) - 1;
+    const Ends& e = sm.ends[sm.order[max(c.start, 0)]];
+    c.b = c.start < 0 ? e.head_b : e.tail_b;
+    c.hc = c.start < 0 ? e.head_hc : e.tail_hc;
+    const unsigned ends = c.start + 1 < 32 ? ending >> (c.start + 1) : 0u;  // the first of the following heads that ends
+    c.ended = ends != 0u;
+    c.links = (c.ended ? c.start + 1 + __ffs(ends) : active) - max(c.start, 0);
+    return c;
+  };
+  for (int task = warp; task < chains * COLS; task += WARPS) {
+    const int local = task % COLS;
+    const Chain ch = chain_of(task / COLS);
+    const Weight w = weight(ch.b);
+    int kvh, column0, row0;
+    place(w, ch.b, ch.hc, kvh, column0, row0);
+    const int c = column0 + local, j = div_small(c, p.inv_group), row = row0 + j;
+    if (j >= min(w.fresh, p.max_new) || row < 0 || row >= p.rows) continue;
+    auto link = [&](int i) -> const float* {
+      const int w = sm.order[max(ch.start, 0) + i];
+      return ch.start >= 0 && i == 0 ? reinterpret_cast<const float*>(sm.ring[w][0]) + local * PARTIAL_FLOATS : sm.head[w][local];
+    };
+    float sum, joined;
+    const float4 v = join_links(ch.links, link, lane, sum, joined);
+    if (ch.start >= 0 && ch.ended) {
+      store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+    } else {
+      float* slot = p.partial + ((static_cast<size_t>(blockIdx.x) * 2 + (ch.start >= 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS;
+      *reinterpret_cast<float4*>(slot + 4 * lane) = v;
+      if (lane == 0) {
+        slot[HEAD_DIM] = joined;
+        slot[HEAD_DIM + 1] = sum;
+      }
+    }
   }
-  const float inv = 1.0f / sum;
-  const bool any = sum != 0.0f;  // no keys: zeros
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? o4[0] * inv : 0.f, any ? o4[1] * inv : 0.f);
-  const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? o4[2] * inv : 0.f, any ? o4[3] * inv : 0.f);
-  *reinterpret_cast<uint2*>(p.out + row * p.ld_out + head * HEAD_DIM + lane * 4) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+
+  // ---- what is cut between CTAs: the first chain if it began in an earlier CTA, the last one if it goes on
+  __syncthreads();
+  const Chain first = chain_of(0), last = chain_of(chains - 1);
+  const bool cut0 = first.start < 0, cut1 = last.start >= 0 && !last.ended;
+  auto span = [&](const Chain& ch, int& c0, int& c1) {  // the CTAs that hold tiles of its segment
+    const unsigned tiles = weight(ch.b).tiles, at = cost_of(prefix[ch.b]) + ch.hc * (tiles + SEGMENT_COST) + SEGMENT_COST;
+    c0 = static_cast<int>(cut.part_of(at));
+    c1 = static_cast<int>(cut.part_of(at + tiles - 1));
+  };
+  if (threadIdx.x < 2 && (threadIdx.x == 0 ? cut0 : cut1)) {
+    int c0, c1;
+    span(threadIdx.x == 0 ? first : last, c0, c1);
+    __threadfence();  // the parts that the other warps wrote before the barrier, too
+    if (atomicAdd(p.arrived + c0, 1) == c1 - c0) {
+      p.arrived[c0] = 0;  // nobody else comes in this launch
+      sm.joins[threadIdx.x] = 1;
+    }
+    __threadfence();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (sm.joins[k] == 0) continue;
+    const Chain& ch = k == 0 ? first : last;
+    int c0, c1;
+    span(ch, c0, c1);
+    const Weight w = weight(ch.b);
+    int kvh, column0, row0;
+    place(w, ch.b, ch.hc, kvh, column0, row0);
+    for (int local = warp; local < COLS; local += WARPS) {
+      const int c = column0 + local, j = div_small(c, p.inv_group), row = row0 + j;
+      if (j >= min(w.fresh, p.max_new) || row < 0 || row >= p.rows) continue;
+      auto link = [&](int i) -> const float* { return p.partial + ((static_cast<size_t>(c0 + i) * 2 + (i == 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS; };
+      float sum, joined;
+      const float4 v = join_links(c1 - c0 + 1, link, lane, sum, joined);
+      store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+    }
+  }
 }
 
 }  // namespace paged
@@ -594,14 +807,13 @@ namespace paged {
 // 8 warps. 16 read the cache once where 8 would read it twice; 8 or fewer columns have no use for the second set.
 constexpr int ATTN_MAX_CTAS = 160;
 constexpr int attn_columns(long long columns) { return columns <= 8 ? 8 : 16; }
-constexpr int attn_warps(int cols) { return cols == 8 ? 16 : 8; }
+constexpr size_t attn_counter_bytes() { return ATTN_MAX_CTAS * sizeof(int); }
+static_assert(attn_counter_bytes() == DF_ATTENTION_PAGED4_COUNTER_BYTES, "the public header's number");
 
 template <int NT, int WARPS, int STAGES>
 int launch_attention(const AttnParams& p, int grid, cudaStream_t s) {
-  constexpr int COLS = 8 * NT;
   using Shared = AttnShared<NT, WARPS, STAGES>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of an SM");
-  static_assert(WARPS == attn_warps(COLS), "the merge launch counts the same workers");
   auto kernel = attention_paged4_kernel<NT, WARPS, STAGES>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
   if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -614,13 +826,6 @@ int launch_attention(const AttnParams& p, int grid, cudaStream_t s) {
   cfg.numAttrs = dependent_launch_attr(&attr);
   cfg.attrs = &attr;
   e = cudaLaunchKernelEx(&cfg, kernel, p);
-  if (e == cudaSuccess) {
-    const long long warps = static_cast<long long>(p.requests) * p.max_new * p.q_heads;
-    cfg.gridDim = dim3(static_cast<unsigned>((warps * 32 + 255) / 256), 1, 1);
-    cfg.blockDim = dim3(256, 1, 1);
-    cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, attention_paged4_merge_kernel<COLS>, p, grid, WARPS);
-  }
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail(DF_ECUDA, "paged attention launch: %s", cudaGetErrorString(e));
@@ -635,8 +840,8 @@ extern "C" size_t df_attention_paged4_workspace_bytes(int requests, int q_heads,
   using namespace df::paged;
   if (requests <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new <= 0 || q_heads % kv_heads != 0) return 0;
   const int cols = attn_columns(static_cast<long long>(max_new) * (q_heads / kv_heads));
-  const size_t partial = static_cast<size_t>(ATTN_MAX_CTAS) * attn_warps(cols) * 2 * cols * PARTIAL_FLOATS * sizeof(float);
-  return partial + ((static_cast<size_t>(requests) + 1) * sizeof(long long) + 15) / 16 * 16;
+  const size_t partial = static_cast<size_t>(ATTN_MAX_CTAS) * 2 * cols * PARTIAL_FLOATS * sizeof(float);
+  return attn_counter_bytes() + static_cast<size_t>(requests + 1) / 2 * 2 * sizeof(uint2) + partial;
 }
 
 extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const void* cache, const int* page_table_dev,
@@ -660,9 +865,11 @@ extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const voi
   const int cols = attn_columns(columns);
   if (static_cast<long long>(max_pages) * page_size > 0x7fffffffLL)
     return fail(DF_EUNSUPPORTED, "max_pages * page_size must stay below 2^31");
-  const long long longest = (static_cast<long long>(max_pages) * (page_size / GRANULE)) * kv_heads;
-  if (columns > 0x7fffffffLL || longest > 0x7fffffffLL / ((columns + cols - 1) / cols))
-    return fail(DF_EUNSUPPORTED, "max_pages * page_size / 16 * kv_heads * ceil(max_new * group / %d) must stay below 2^31", cols);
+  // the list of tiles is numbered with 32 bits
+  const double most = static_cast<double>(requests) * (static_cast<double>(max_pages) * page_size / TILE + 1 + SEGMENT_COST) * kv_heads *
+                      static_cast<double>((columns + cols - 1) / cols);
+  if (columns >= MAX_COLUMNS || kv_heads >= MAX_COLUMNS || most >= 2147483648.0)
+    return fail(DF_EUNSUPPORTED, "requests * (max_pages * page_size / %d + %u) * kv_heads * ceil(max_new * group / %d) must stay below 2^31", TILE, SEGMENT_COST + 1, cols);
   if (static_cast<long long>(requests) * max_new > 0x7fffffffLL / q_heads / 4)
     return fail(DF_EUNSUPPORTED, "requests * max_new * q_heads must stay below 2^29");
   if (ld_q < static_cast<long long>(q_heads) * HEAD_DIM || ld_out < static_cast<long long>(q_heads) * HEAD_DIM || (ld_q % 8) != 0 || (ld_out % 8) != 0)
@@ -684,9 +891,9 @@ extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const voi
   p.row_starts = row_starts_dev;
   p.new_lens = new_lens_dev;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.prefix = static_cast<long long*>(workspace);
-  // the partial results start at a multiple of 16 bytes behind the prefix sums
-  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((static_cast<size_t>(requests) + 1) * sizeof(long long) + 15) / 16 * 16);
+  p.arrived = static_cast<int*>(workspace);
+  p.prefix = reinterpret_cast<uint2*>(static_cast<uint8_t*>(workspace) + attn_counter_bytes());
+  p.partial = reinterpret_cast<float*>(p.prefix + (requests + 1) / 2 * 2);
   p.ld_q = ld_q;
   p.ld_out = ld_out;
   p.rows = rows;
@@ -699,8 +906,9 @@ extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const voi
   p.group = q_heads / kv_heads;
   p.max_new = max_new;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.inv_group = 1.0f / static_cast<float>(p.group);
   p.timeout_ns = timeout_ns();
   p.status = reinterpret_cast<Status*>(dev_status);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cols == 8 ? launch_attention<1, 16, 6>(p, grid, s) : launch_attention<2, 8, 12>(p, grid, s);
+  return cols == 8 ? launch_attention<1, 16, 2>(p, grid, s) : launch_attention<2, 12, 2>(p, grid, s);
 }

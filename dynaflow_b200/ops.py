@@ -446,12 +446,12 @@ def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.
 
 def attention_paged4_workspace(requests: int, q_heads: int, kv_heads: int, max_new: int = 1,
                                device: torch.device | str = "cuda") -> torch.Tensor:
-    """Scratch for ``attention_paged4`` (partial results of cut requests); its contents are arbitrary. Calls that can overlap
-    on the GPU, captured graphs included, need one each."""
+    """Scratch for ``attention_paged4`` (partial results of cut requests), zeroed: its counters are zero between calls. Calls
+    that can overlap on the GPU, captured graphs included, need one each."""
     need = int(_native.load().df_attention_paged4_workspace_bytes(requests, q_heads, kv_heads, max_new))
     if need == 0:
         raise ValueError("requests, max_new and the head counts must be positive, q_heads a multiple of kv_heads")
-    return torch.empty(need, dtype=torch.uint8, device=device)
+    return torch.zeros(need, dtype=torch.uint8, device=device)
 
 
 def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, out: torch.Tensor,

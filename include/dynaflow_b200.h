@@ -511,8 +511,10 @@ int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, void* out, lon
  * NULL: one row a request, row b); row j of them attends keys 0 .. seq_lens[b] - new_lens[b] + j, query head h reads
  * key/value head h / (q_heads / kv_heads). Keys whose page is missing (page_table outside [0, num_pages)) do not count;
  * a row without keys is zeros. Rows of no request are left as they were. `workspace`: device scratch of
- * df_attention_paged4_workspace_bytes(), contents arbitrary, one for launches that can overlap. max_ctas limits the
- * launch to that many SMs (0: all). Reproducible bit for bit at a given max_ctas. */
+ * df_attention_paged4_workspace_bytes(), whose first DF_ATTENTION_PAGED4_COUNTER_BYTES are zero before its first use (a
+ * launch leaves them zero; after a status error zero them again); one for launches that can overlap. max_ctas limits
+ * the launch to that many SMs (0: all). Reproducible bit for bit at a given max_ctas. */
+#define DF_ATTENTION_PAGED4_COUNTER_BYTES 640
 size_t df_attention_paged4_workspace_bytes(int requests, int q_heads, int kv_heads, int max_new);
 int df_attention_paged4_bf16(const void* q, long long ld_q, const void* cache, const int* page_table_dev,
                              const int* seq_lens_dev, const int* row_starts_dev, const int* new_lens_dev, void* out,

@@ -98,7 +98,7 @@ def _run(ops, case, q, group, *, fresh=None, starts=None, max_new=1, scale=None,
     out_room = torch.full((rows, cols + wide), 7.0, dtype=torch.bfloat16, device="cuda")
     out = out_room[:, :cols]
     ws = ops.attention_paged4_workspace(len(case.lens), hq, case.hkv, max_new)
-    ws.fill_(0xFF)
+    ws[640:].fill_(0xFF)                 # all but the counters
     more = dict(row_starts=_i32(starts), new_lens=_i32(fresh), max_new=max_new) if fresh is not None else {}
     args = (room[:, :cols], case.cache.cuda(), _i32(page_table or case.table), _i32(case.lens), out, ws)
     ops.attention_paged4(*args, page_size=case.page, scale=scale, max_ctas=max_ctas, **more)
