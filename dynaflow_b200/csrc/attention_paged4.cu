@@ -52,6 +52,7 @@ constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and pref
 constexpr int TILE = 2 * GRANULE;             // tokens
 constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
 constexpr unsigned SEGMENT_COST = 2;          // tiles
+constexpr unsigned JOIN_COST = 40;            // tiles of 8 columns a CTA does in the time that a join between CTAs takes
 constexpr int MAX_COLUMNS = 1 << 20;
 
 struct AttnParams {
@@ -159,8 +160,8 @@ __device__ __forceinline__ float max_rows(float v) {
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
-// A tile in the ring. `flags`: tile of the segment << 3, whether its segment's first tile of this part, whether each
-// of its granules has a page.
+// A tile in the ring. `flags`: tile of the segment << 3, whether a segment begins with it (but for the part's
+// first tile), whether each of its granules has a page.
 struct Desc {
   int flags, b, hc;  // request, key/value head * blocks + block
 };
@@ -183,6 +184,7 @@ struct AttnShared {
   uint2 prefix[REQUESTS_IN_SMEM];
   int2 lens[REQUESTS_IN_SMEM];                   // length, new tokens
   uint2 warp_sum[WARPS];
+  unsigned warp_longest[WARPS];
   Ends ends[WARPS];
   int order[WARPS];                              // the warps that have tiles
   uint32_t abort;
@@ -242,6 +244,7 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* dst, float4 v, float su
 template <int NT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const AttnParams p) {
   constexpr int COLS = 8 * NT, THREADS = WARPS * 32;
+  constexpr int HN = NT == 1 ? 2 : 1;  // granules gone through together: as many as the registers hold
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<AttnShared<NT, WARPS, STAGES>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   const bool in_smem = p.requests <= REQUESTS_IN_SMEM;
   uint2* prefix = in_smem ? sm.prefix : p.prefix;
   uint2 all{0, 0};
+  unsigned longest = 0;  // tiles
   for (int b0 = 0; b0 < p.requests; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
     uint2 v{0, 0};
@@ -265,6 +269,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       v.y = static_cast<unsigned>(w.blocks) * p.kv_heads;
       v.x = v.y * w.tiles;
       if (in_smem) sm.lens[b] = make_int2(w.len, w.fresh);
+      if (w.blocks > 0) longest = max(longest, static_cast<unsigned>(w.tiles));
     }
     uint2 inc = v;
 #pragma unroll
@@ -275,13 +280,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         inc.y += uy;
       }
     }
+    longest = __reduce_max_sync(0xffffffffu, longest);
     if (b0 > 0) __syncthreads();
-    if (lane == 31) sm.warp_sum[warp] = inc;
+    if (lane == 31) {
+      sm.warp_sum[warp] = inc;
+      sm.warp_longest[warp] = longest;
+    }
     __syncthreads();
     uint2 before = all;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
       const uint2 s = sm.warp_sum[i];
+      longest = max(longest, sm.warp_longest[i]);
       if (i < warp) {
         before.x += s.x;
         before.y += s.y;
@@ -294,7 +304,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   if (all.x == 0) return;
   const unsigned cost = cost_of(all);
   const Cut cut(cost, min(static_cast<unsigned>(gridDim.x), (cost + WARPS - 1) / WARPS));
-  if (blockIdx.x >= cut.parts) return;
+  // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
+  // head, on 148 CTAs: 23.2 us against 27.1 us cut evenly)
+  const unsigned per_cta = (all.y + gridDim.x - 1) / gridDim.x;
+  const bool whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
+  const unsigned parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;
+  if (blockIdx.x >= parts) return;
   if (threadIdx.x < 2) sm.joins[threadIdx.x] = 0;
   __syncthreads();
 
@@ -308,33 +323,49 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     }
     return lo;
   };
-  // tiles that lie before a place of the list given as cost
+  // tiles that lie before a place of the list given as cost, and the request that the place is in
+  int cut_b = 0;
   auto tiles_before = [&](unsigned at) {
     if (at >= cost) return all.x;
-    const int b = find(at, [](const uint2& v) { return cost_of(v); });
-    const unsigned tiles = weight(b).tiles, rel = at - cost_of(prefix[b]), each = tiles + SEGMENT_COST;
+    cut_b = find(at, [](const uint2& v) { return cost_of(v); });
+    const unsigned tiles = weight(cut_b).tiles, rel = at - cost_of(prefix[cut_b]), each = tiles + SEGMENT_COST;
     const unsigned s = rel / each, in = rel - s * each;
-    return prefix[b].x + s * tiles + (in > SEGMENT_COST ? in - SEGMENT_COST : 0u);
+    return prefix[cut_b].x + s * tiles + (in > SEGMENT_COST ? in - SEGMENT_COST : 0u);
   };
-  // the parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins
-  const unsigned at0 = cut.start(blockIdx.x), at_n = cut.start(blockIdx.x + 1) - at0;
+  auto part_start = [&](unsigned c) {
+    if (!whole) return cut.start(c);
+    const unsigned s = c * per_cta;
+    if (s >= all.y) return cost;
+    const int b = find(s, [](const uint2& v) { return v.y; });
+    return cost_of(prefix[b]) + (s - prefix[b].y) * (static_cast<unsigned>(weight(b).tiles) + SEGMENT_COST);
+  };
+  // the parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins. (Every warp has the queries of
+  // its first segment to fetch: the CTA's first segment costs nothing more.)
+  const unsigned bound = part_start(blockIdx.x + (lane & 1));
+  const unsigned at0 = __shfl_sync(0xffffffffu, bound, 0) + (whole ? SEGMENT_COST : 0u), at_n = __shfl_sync(0xffffffffu, bound, 1) - at0;
   const unsigned cut_at = tiles_before(at0 + Cut(at_n, WARPS).start(min(lane, WARPS)));
   const unsigned f0 = __shfl_sync(0xffffffffu, cut_at, warp);
   const int count = static_cast<int>(__shfl_sync(0xffffffffu, cut_at, warp + 1) - f0);
+  int cur_b = __shfl_sync(0xffffffffu, cut_b, warp);  // request of the part's first tile, then of the last look-up's first
+  auto request_of = [&](int b, unsigned f) {  // of tile f, from a request at or before it
+    while (b + 1 < p.requests && prefix[b + 1].x <= f) ++b;
+    return b;
+  };
 
   // ---- copies: lane i looks up the i-th of the next 32 tiles; `issue(s)` starts the copies of its tile into stage s
   Desc ahead{0, 0, 0};
   const uint8_t* ahead_src[2] = {nullptr, nullptr};
   auto look_up = [&](int n) {
+    cur_b = request_of(cur_b, f0 + n);
     if (n + lane < count) {
       const unsigned f = f0 + n + lane;
-      const int b = find(f, [](const uint2& v) { return v.x; });
+      const int b = request_of(cur_b, f);
       const Weight w = weight(b);
       const unsigned rel = f - prefix[b].x, hc = rel / w.tiles;
       const int tile = static_cast<int>(rel - hc * w.tiles);
       ahead.b = b;
       ahead.hc = static_cast<int>(hc);
-      ahead.flags = tile << 3 | (tile == 0 || n + lane == 0 ? TILE_FIRST : 0);
+      ahead.flags = tile << 3 | (tile == 0 && n + lane > 0 ? TILE_FIRST : 0);
       const int kvh = w.blocks == 1 ? ahead.hc : ahead.hc / w.blocks;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -364,9 +395,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       if ((ahead.flags & 2) != 0) bulk_load(dst + GRANULE_BYTES, ahead_src[1], GRANULE_BYTES, bar);
     }
   };
-  look_up(0);
-  if (lane < STAGES && lane < count) issue(lane);
-  __syncwarp();
 
   // ---- state of the segment (one request, key/value head and set of columns)
   uint32_t qf[NT][16];                        // Q^T fragments: pair p of the 16 this thread's 32 dimensions make
@@ -387,6 +415,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     row0 = p.row_starts != nullptr ? p.row_starts[b] : b;
   };
 
+  uint4 raw[NT][4];
+  auto load_queries = [&](int b, int hc) {  // this lane's 32 dimensions of column g of each set
+    const Weight w = weight(b);
+    int kvh, column0, row0;
+    place(w, b, hc, kvh, column0, row0);
+    const int served = min(w.fresh, p.max_new);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = column0 + nt * 8 + g, j = div_small(c, p.inv_group), row = row0 + j;
+      const bool here = j < served && row >= 0 && row < p.rows;
+      const __nv_bfloat16* src = p.q + row * p.ld_q + (kvh * p.group + c - j * p.group) * HEAD_DIM + t * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[nt][i] = here ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
   auto begin = [&](int b, int hc, int tile) {
     seg_b = b;
     seg_hc = hc;
@@ -401,18 +444,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     v_exp = -100;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int c = column0 + nt * 8 + g;  // this lane's column of the B fragments
-      const int j = div_small(c, p.inv_group), row = row0 + j;
-      const bool here = j < served && row >= 0 && row < p.rows;
-      uint4 raw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        raw[i] = here ? *reinterpret_cast<const uint4*>(p.q + row * p.ld_q + (kvh * p.group + c - j * p.group) * HEAD_DIM + t * 32 + i * 8)
-                      : make_uint4(0u, 0u, 0u, 0u);
       float x[32], big = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        const uint32_t w4[4] = {raw[nt][i].x, raw[nt][i].y, raw[nt][i].z, raw[nt][i].w};
         float most = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -514,12 +549,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   const uint32_t lm_off = HALF_GRANULE + lm_row * CODE_BYTES + (chunk_place(lane >> 4, lm_row) << 4);
   const uint32_t k_off = g * CODE_BYTES + (chunk_place(t, g) << 4);
 
+  // the first queries are on their way while the pages are looked up and the first copies start
+  if (count > 0) {
+    const int b = cur_b = request_of(cur_b, f0);
+    const unsigned tiles = weight(b).tiles, rel = f0 - prefix[b].x, hc = rel / tiles;
+    load_queries(b, static_cast<int>(hc));
+    look_up(0);
+    if (lane < STAGES && lane < count) issue(lane);
+    __syncwarp();
+    begin(b, static_cast<int>(hc), static_cast<int>(rel - hc * tiles));
+  }
   bool ok = true;
   int stage = 0, phase = 0, base = 0;  // ring position of tile n; first tile of the last look-up
   for (int n = 0; n < count; ++n) {
     const int flags = sm.desc[warp][stage].flags, tile = flags >> 3;
     if ((flags & TILE_FIRST) != 0) {
-      if (n > 0) flush();
+      flush();
+      load_queries(sm.desc[warp][stage].b, sm.desc[warp][stage].hc);
       begin(sm.desc[warp][stage].b, sm.desc[warp][stage].hc, tile);
     }
     seg_last = tile;
@@ -532,11 +578,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     const uint8_t* st = sm.ring[warp][stage];
     const bool edge = (flags & TILE_PAGES) != TILE_PAGES || (tile + 1) * TILE > min_limit;
 
+#pragma unroll 1
+    for (int h0 = 0; h0 < 2; h0 += HN) {
     // ---- S^T = K Q^T
-    float sc[2][NT][4];
+    float sc[HN][NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 ka = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off), kb = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off + 8 * CODE_BYTES);
+    for (int h = 0; h < HN; ++h) {
+      const uint4 ka = *reinterpret_cast<const uint4*>(st + (h0 + h) * GRANULE_BYTES + k_off), kb = *reinterpret_cast<const uint4*>(st + (h0 + h) * GRANULE_BYTES + k_off + 8 * CODE_BYTES);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -550,13 +598,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       }
     }
     // ---- scores less their reference, log2
-    float vs[2][2], vm[2][2];
+    float vs[HN][2], vm[HN][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < HN; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + PARAM_OFFSET + (g + 8 * r) * 4);
-        const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
+        const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + (h0 + h) * GRANULE_BYTES + PARAM_OFFSET + (g + 8 * r) * 4);
+        const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + (h0 + h) * GRANULE_BYTES + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
         const float ks = __uint_as_float(kp << 16), km = __uint_as_float(kp & 0xffff0000u);
         vs[h][r] = __uint_as_float(vp << 16);
         vm[h][r] = __uint_as_float(vp & 0xffff0000u);
@@ -571,11 +619,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     bool careful = false;  // a key that only some columns see has parameters that are no numbers
     if (edge) {            // masked keys: no score, and parameters (whatever lies there) that count for nothing
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < HN; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const bool page = (flags >> h & 1) != 0;
-          const int key = tile * TILE + h * GRANULE + g + 8 * r;
+          const bool page = (flags >> (h0 + h) & 1) != 0;
+          const int key = tile * TILE + (h0 + h) * GRANULE + g + 8 * r;
           bool any = false, every = true;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -591,14 +639,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         }
       careful = __any_sync(0xffffffffu, careful);
     }
-    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[HN - 1][0], vs[HN - 1][1]));
     float top[NT][2];
     bool move = vmax > v_limit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
+        top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[HN - 1][nt][c], sc[HN - 1][nt][2 + c]));
         move = move || top[nt][c] > over[nt][c];
       }
     if (__any_sync(0xffffffffu, move)) {
@@ -630,7 +678,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             acc[nt][i][2 + c] *= both;
           }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < HN; ++h) {
             sc[h][nt][c] -= rise;
             sc[h][nt][2 + c] -= rise;
           }
@@ -638,7 +686,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     }
     // ---- P^T, then O^T += V^T P^T
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < HN; ++h) {
       uint32_t pf[NT][2];
       const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * v_scale};
 #pragma unroll
@@ -664,7 +712,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
       }
-      const uint32_t st_addr = smem_u32(st) + h * GRANULE_BYTES;
+      const uint32_t st_addr = smem_u32(st) + (h0 + h) * GRANULE_BYTES;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t v[4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
@@ -679,6 +727,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
           }
         }
       }
+    }
     }
     __syncwarp();  // every lane has read the stage
     const int next = n + STAGES;
@@ -757,6 +806,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     }
   }
 
+  if (whole) return;
   // ---- what is cut between CTAs: the first chain if it began in an earlier CTA, the last one if it goes on
   __syncthreads();
   const Chain first = chain_of(0), last = chain_of(chains - 1);
