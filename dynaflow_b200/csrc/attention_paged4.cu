@@ -63,7 +63,8 @@ struct AttnParams {
   const int* row_starts;  // may be null: request b is row b
   const int* new_lens;    // may be null: one row a request
   __nv_bfloat16* out;
-  float* partial;         // [ctas][2][columns][PARTIAL_FLOATS]
+  float* partial;         // [ctas][2][columns][PARTIAL_FLOATS]: what CTAs leave
+  float* heads;           // [ctas][warps][columns][PARTIAL_FLOATS]: what warps leave before their end
   int* arrived;           // [ctas] CTAs that have left their part of the request and head whose first part is CTA c's; zero between launches
   uint2* prefix;          // [requests] what lies before a request: tiles, segments
   long long ld_q, ld_out;
@@ -168,20 +169,30 @@ struct Desc {
 constexpr int TILE_FIRST = 4, TILE_PAGES = 3;
 
 // What a warp leaves of requests it does not hold whole: `head` began in an earlier warp, `tail` goes on in a later one.
+// The last thing that a warp leaves lies in its ring, a head that it goes on from in p.heads.
 struct Ends {
   int head_b, head_hc, head_ends;  // head_b < 0: none; head_ends: its last tile is in this warp
+  int head_in_ring;
   int tail_b, tail_hc;             // tail_b < 0: none
   int used;                        // whether the warp has tiles
+};
+
+// Q^T fragments of a segment, of every lane: the four pairs of each word of its 16 bytes.
+template <int NT>
+struct Queries {
+  uint4 qf[NT][4][32];
 };
 
 template <int NT, int WARPS, int STAGES>
 struct AttnShared {
   static constexpr int COLS = 8 * NT;
-  uint8_t ring[WARPS][STAGES][TILE_BYTES];       // at the end a warp's tail lies in its own ring
-  float head[WARPS][COLS][PARTIAL_FLOATS];
+  uint8_t ring[WARPS][STAGES][TILE_BYTES];       // at the end: what a warp leaves
   Desc desc[WARPS][STAGES];
   uint64_t full[WARPS][STAGES];
   uint2 prefix[REQUESTS_IN_SMEM];
+  uint2 part[WARPS + 1];                         // first tile of a warp's part and its request
+  Queries<NT> queries[WARPS + 1];                // of the warps' segments; the last: of the CTA's first segment
+  float2 column[NT][2][32];                      // c1 and sq of the CTA's first segment, of every lane
   int2 lens[REQUESTS_IN_SMEM];                   // length, new tokens
   uint2 warp_sum[WARPS];
   unsigned warp_longest[WARPS];
@@ -189,7 +200,7 @@ struct AttnShared {
   int order[WARPS];                              // the warps that have tiles
   uint32_t abort;
   int joins[2];                                  // whether this CTA joins the parts of its first / last segment
-  static_assert(STAGES * TILE_BYTES >= COLS * PARTIAL_FLOATS * 4, "the tail fits into the ring");
+  static_assert(STAGES * TILE_BYTES >= COLS * PARTIAL_FLOATS * 4, "a partial result fits into the ring");
 };
 
 // Weighted sum of one column of the partial results `link(i)`, i in [0, n): lane l has dimensions 4l .. 4l + 3.
@@ -244,7 +255,6 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* dst, float4 v, float su
 template <int NT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const AttnParams p) {
   constexpr int COLS = 8 * NT, THREADS = WARPS * 32;
-  constexpr int HN = NT == 1 ? 2 : 1;  // granules gone through together: as many as the registers hold
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<AttnShared<NT, WARPS, STAGES>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -280,16 +290,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         inc.y += uy;
       }
     }
-    longest = __reduce_max_sync(0xffffffffu, longest);
     if (b0 > 0) __syncthreads();
+    longest = __reduce_max_sync(0xffffffffu, longest);
     if (lane == 31) {
       sm.warp_sum[warp] = inc;
       sm.warp_longest[warp] = longest;
     }
     __syncthreads();
     uint2 before = all;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
+    const int holding = min(WARPS, (p.requests - b0 + 31) >> 5);  // warps with a request
+    for (int i = 0; i < holding; ++i) {
       const uint2 s = sm.warp_sum[i];
       longest = max(longest, sm.warp_longest[i]);
       if (i < warp) {
@@ -341,12 +351,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   };
   // the parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins. (Every warp has the queries of
   // its first segment to fetch: the CTA's first segment costs nothing more.)
-  const unsigned bound = part_start(blockIdx.x + (lane & 1));
-  const unsigned at0 = __shfl_sync(0xffffffffu, bound, 0) + (whole ? SEGMENT_COST : 0u), at_n = __shfl_sync(0xffffffffu, bound, 1) - at0;
-  const unsigned cut_at = tiles_before(at0 + Cut(at_n, WARPS).start(min(lane, WARPS)));
-  const unsigned f0 = __shfl_sync(0xffffffffu, cut_at, warp);
-  const int count = static_cast<int>(__shfl_sync(0xffffffffu, cut_at, warp + 1) - f0);
-  int cur_b = __shfl_sync(0xffffffffu, cut_b, warp);  // request of the part's first tile, then of the last look-up's first
+  if (warp == 0) {
+    const unsigned bound = part_start(blockIdx.x + (lane & 1));
+    const unsigned at0 = __shfl_sync(0xffffffffu, bound, 0) + (whole ? SEGMENT_COST : 0u), at_n = __shfl_sync(0xffffffffu, bound, 1) - at0;
+    const unsigned cut_at = tiles_before(at0 + Cut(at_n, WARPS).start(min(lane, WARPS)));
+    if (lane <= WARPS) sm.part[lane] = make_uint2(cut_at, cut_b);
+  }
+  __syncthreads();
+  const unsigned f0 = sm.part[warp].x;
+  const int count = static_cast<int>(sm.part[warp + 1].x - f0);
+  int cur_b = static_cast<int>(sm.part[warp].y);  // request of the part's first tile, then of the last look-up's first
   auto request_of = [&](int b, unsigned f) {  // of tile f, from a request at or before it
     while (b + 1 < p.requests && prefix[b + 1].x <= f) ++b;
     return b;
@@ -397,7 +411,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   };
 
   // ---- state of the segment (one request, key/value head and set of columns)
-  uint32_t qf[NT][16];                        // Q^T fragments: pair p of the 16 this thread's 32 dimensions make
+  uint4 qf[NT == 1 ? 4 : 1];                  // Q^T fragments; with two sets of columns they stay in shared memory
+  int query_slot = warp;
   float c1[NT][2], sq[NT][2];                 // score = (acc s_k + sq m_k) c1, of columns 2t and 2t + 1
   int limit[NT][2];                           // keys a column sees
   float ref[NT][2], over[NT][2];              // reference (log2); a score that exceeds it by `over` moves it (-inf: none yet)
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   float v_scale = 1.0f, v_limit = -1.0f;      // p s_v is held times v_scale = 2^-v_exp; scales above v_limit move it
   int v_exp = -100;
   int seg_b = -1, seg_hc = 0, seg_first = 0, seg_last = 0, min_limit = 0;
-  Ends ends{-1, -1, 0, -1, -1, count > 0 ? 1 : 0};
+  Ends ends{-1, -1, 0, 0, -1, -1, count > 0 ? 1 : 0};
 
   // head, first column and first row of a segment
   auto place = [&](const Weight& w, int b, int hc, int& kvh, int& column0, int& row0) {
@@ -430,18 +445,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       for (int i = 0; i < 4; ++i) raw[nt][i] = here ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  auto begin = [&](int b, int hc, int tile) {
-    seg_b = b;
-    seg_hc = hc;
-    seg_first = tile;
-    const Weight w = weight(b);
-    int kvh, column0, row0;
-    place(w, b, hc, kvh, column0, row0);
-    const int served = min(w.fresh, p.max_new);
-    min_limit = w.len;
-    v_scale = 1.0f;
-    v_limit = -1.0f;
-    v_exp = -100;
+  auto make_fragments = [&](int slot) {  // from the queries that were loaded
+    auto& to = sm.queries[slot];
+    query_slot = slot;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[32], big = 0.f;
@@ -461,27 +467,54 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       const int e = max(min(exponent_of(big), 117), -100);
       const float up[2] = {pow2i(14 - e), pow2i(10 - e)};
+      uint32_t f[16];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // word i of the 16 bytes, nibbles k and k + 4: dimensions 8i + k and 8i + k + 4 (odd k: 16 times the code)
           const __half2 h = __floats2half2_rn(x[i * 8 + k] * up[k & 1], x[i * 8 + k + 4] * up[k & 1]);
-          qf[nt][i * 4 + k] = *reinterpret_cast<const uint32_t*>(&h);
+          f[i * 4 + k] = *reinterpret_cast<const uint32_t*>(&h);
         }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to.qf[nt][i][lane] = make_uint4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
       // the sum of q: its product with codes that are all one
       float one[4];
-      mma_f16_first(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[nt][0], qf[nt][1]);
+      mma_f16_first(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, f[0], f[1]);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mma_f16(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[nt][2 * i], qf[nt][2 * i + 1]);
+      for (int i = 1; i < 8; ++i) mma_f16(one, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, f[2 * i], f[2 * i + 1]);
       const float a = p.scale_log2 * pow2i(e + 10);  // 2^24 of the codes, 2^(e - 14) of q
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int cc = 2 * t + k;  // the columns of this thread's scores: held by lane group cc
-        c1[nt][k] = __shfl_sync(0xffffffffu, a, cc * 4);
+        c1[nt][k] = __shfl_sync(0xffffffffu, a, (2 * t + k) * 4);  // the columns of this thread's scores: held by lane group 2t + k
         sq[nt][k] = one[k];
-        const int jj = div_small(column0 + nt * 8 + cc, p.inv_group);
-        limit[nt][k] = jj < served ? min(w.len - w.fresh + jj + 1, w.len) : w.len;  // a column without a query is computed and dropped
+      }
+    }
+    __syncwarp();
+  };
+  auto hold_fragments = [&]() {
+    if (NT == 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[i < NT * 4 ? i : 0] = sm.queries[query_slot].qf[0][i][lane];
+  };
+  auto begin = [&](int b, int hc, int tile) {  // everything of a segment's state but the fragments
+    seg_b = b;
+    seg_hc = hc;
+    seg_first = tile;
+    const Weight w = weight(b);
+    int kvh, column0, row0;
+    place(w, b, hc, kvh, column0, row0);
+    const int served = min(w.fresh, p.max_new);
+    min_limit = w.len;
+    v_scale = 1.0f;
+    v_limit = -1.0f;
+    v_exp = -100;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int j = div_small(column0 + nt * 8 + 2 * t + k, p.inv_group);
+        limit[nt][k] = j < served ? min(w.len - w.fresh + j + 1, w.len) : w.len;  // a column without a query is computed and dropped
         ref[nt][k] = 0.f;
         over[nt][k] = -INFINITY;
         l[nt][k] = 0.f;
@@ -497,7 +530,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     for (int o = 1; o < 4; o <<= 1) min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, o));
   };
 
-  auto flush = [&]() {
+  auto flush = [&](bool last) {
     const Weight w = weight(seg_b);
     const bool began = seg_first == 0, ended = seg_last == w.tiles - 1;
     int kvh, column0, row0;
@@ -505,15 +538,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     const int served = min(w.fresh, p.max_new);
     const float back = 16777216.0f * pow2i(v_exp);  // 2^24 of the codes
     float* part = nullptr;
-    if (!began) {
-      part = sm.head[warp][0];
-      ends.head_b = seg_b;
-      ends.head_hc = seg_hc;
-      ends.head_ends = ended;
-    } else if (!ended) {  // the last segment of the part: every copy into the ring has been read
-      part = reinterpret_cast<float*>(sm.ring[warp][0]);
-      ends.tail_b = seg_b;
-      ends.tail_hc = seg_hc;
+    if (!began || !ended) {
+      part = last ? reinterpret_cast<float*>(sm.ring[warp][0])  // every copy into the ring has been read
+                  : p.heads + (static_cast<size_t>(blockIdx.x) * WARPS + warp) * COLS * PARTIAL_FLOATS;
+      if (!began) {
+        ends.head_b = seg_b;
+        ends.head_hc = seg_hc;
+        ends.head_ends = ended;
+        ends.head_in_ring = last;
+      } else {
+        ends.tail_b = seg_b;
+        ends.tail_hc = seg_hc;
+      }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -549,23 +585,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   const uint32_t lm_off = HALF_GRANULE + lm_row * CODE_BYTES + (chunk_place(lane >> 4, lm_row) << 4);
   const uint32_t k_off = g * CODE_BYTES + (chunk_place(t, g) << 4);
 
-  // the first queries are on their way while the pages are looked up and the first copies start
+  // The first queries are on their way while the pages are looked up and the first copies start. Warps that begin in the
+  // CTA's first segment (all of them where requests are long) take its fragments from the first warp.
+  int first_b = 0, first_hc = 0, first_tile = 0;
+  bool shared_queries = false;
   if (count > 0) {
-    const int b = cur_b = request_of(cur_b, f0);
-    const unsigned tiles = weight(b).tiles, rel = f0 - prefix[b].x, hc = rel / tiles;
-    load_queries(b, static_cast<int>(hc));
+    first_b = cur_b = request_of(cur_b, f0);
+    const unsigned tiles = weight(first_b).tiles, rel = f0 - prefix[first_b].x;
+    first_hc = static_cast<int>(rel / tiles);
+    first_tile = static_cast<int>(rel) - first_hc * static_cast<int>(tiles);
+    shared_queries = warp > 0 && f0 - first_tile <= sm.part[0].x && sm.part[1].x > sm.part[0].x;  // the segment began at or before the CTA's first tile
+    if (!shared_queries) load_queries(first_b, first_hc);
     look_up(0);
     if (lane < STAGES && lane < count) issue(lane);
     __syncwarp();
-    begin(b, static_cast<int>(hc), static_cast<int>(rel - hc * tiles));
+    begin(first_b, first_hc, first_tile);
+    if (!shared_queries) make_fragments(warp == 0 ? WARPS : warp);
+    if (warp == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sm.column[nt][k][lane] = make_float2(c1[nt][k], sq[nt][k]);
+    }
   }
+  __syncthreads();
+  if (shared_queries) {
+    query_slot = WARPS;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 v = sm.column[nt][k][lane];
+        c1[nt][k] = v.x;
+        sq[nt][k] = v.y;
+      }
+  }
+  hold_fragments();
   bool ok = true;
   int stage = 0, phase = 0, base = 0;  // ring position of tile n; first tile of the last look-up
   for (int n = 0; n < count; ++n) {
     const int flags = sm.desc[warp][stage].flags, tile = flags >> 3;
     if ((flags & TILE_FIRST) != 0) {
-      flush();
+      flush(false);
       load_queries(sm.desc[warp][stage].b, sm.desc[warp][stage].hc);
+      make_fragments(warp);
+      hold_fragments();
       begin(sm.desc[warp][stage].b, sm.desc[warp][stage].hc, tile);
     }
     seg_last = tile;
@@ -578,33 +642,42 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     const uint8_t* st = sm.ring[warp][stage];
     const bool edge = (flags & TILE_PAGES) != TILE_PAGES || (tile + 1) * TILE > min_limit;
 
-#pragma unroll 1
-    for (int h0 = 0; h0 < 2; h0 += HN) {
     // ---- S^T = K Q^T
-    float sc[HN][NT][4];
+    float sc[2][NT][4];
+    {
+      uint4 ka[2], kb[2];
 #pragma unroll
-    for (int h = 0; h < HN; ++h) {
-      const uint4 ka = *reinterpret_cast<const uint4*>(st + (h0 + h) * GRANULE_BYTES + k_off), kb = *reinterpret_cast<const uint4*>(st + (h0 + h) * GRANULE_BYTES + k_off + 8 * CODE_BYTES);
-      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      for (int h = 0; h < 2; ++h) {
+        ka[h] = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off);
+        kb[h] = *reinterpret_cast<const uint4*>(st + h * GRANULE_BYTES + k_off + 8 * CODE_BYTES);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a8 = wa[i] >> 8, b8 = wb[i] >> 8;
+        uint4 q[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (i == 0) mma_f16_first(sc[h][nt], code_lo(wa[i]), code_lo(wb[i]), code_hi(wa[i]), code_hi(wb[i]), qf[nt][4 * i], qf[nt][4 * i + 1]);
-          else mma_f16(sc[h][nt], code_lo(wa[i]), code_lo(wb[i]), code_hi(wa[i]), code_hi(wb[i]), qf[nt][4 * i], qf[nt][4 * i + 1]);
-          mma_f16(sc[h][nt], code_lo(a8), code_lo(b8), code_hi(a8), code_hi(b8), qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+        for (int nt = 0; nt < NT; ++nt) q[nt] = NT == 1 ? qf[NT == 1 ? i : 0] : sm.queries[query_slot].qf[nt][i][lane];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t wa = i == 0 ? ka[h].x : i == 1 ? ka[h].y : i == 2 ? ka[h].z : ka[h].w;
+          const uint32_t wb = i == 0 ? kb[h].x : i == 1 ? kb[h].y : i == 2 ? kb[h].z : kb[h].w;
+          const uint32_t a8 = wa >> 8, b8 = wb >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (i == 0) mma_f16_first(sc[h][nt], code_lo(wa), code_lo(wb), code_hi(wa), code_hi(wb), q[nt].x, q[nt].y);
+            else mma_f16(sc[h][nt], code_lo(wa), code_lo(wb), code_hi(wa), code_hi(wb), q[nt].x, q[nt].y);
+            mma_f16(sc[h][nt], code_lo(a8), code_lo(b8), code_hi(a8), code_hi(b8), q[nt].z, q[nt].w);
+          }
         }
       }
     }
     // ---- scores less their reference, log2
-    float vs[HN][2], vm[HN][2];
+    float vs[2][2], vm[2][2];
 #pragma unroll
-    for (int h = 0; h < HN; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + (h0 + h) * GRANULE_BYTES + PARAM_OFFSET + (g + 8 * r) * 4);
-        const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + (h0 + h) * GRANULE_BYTES + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
+        const uint32_t kp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + PARAM_OFFSET + (g + 8 * r) * 4);
+        const uint32_t vp = *reinterpret_cast<const uint32_t*>(st + h * GRANULE_BYTES + HALF_GRANULE + PARAM_OFFSET + (g + 8 * r) * 4);
         const float ks = __uint_as_float(kp << 16), km = __uint_as_float(kp & 0xffff0000u);
         vs[h][r] = __uint_as_float(vp << 16);
         vm[h][r] = __uint_as_float(vp & 0xffff0000u);
@@ -616,37 +689,44 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             x = fmaf(fmaf(x, ks, sq[nt][c] * km), c1[nt][c], -ref[nt][c]);
           }
       }
-    bool careful = false;  // a key that only some columns see has parameters that are no numbers
-    if (edge) {            // masked keys: no score, and parameters (whatever lies there) that count for nothing
+    if (edge) {  // masked keys: no score, and parameters (whatever lies there) that count for nothing
 #pragma unroll
-      for (int h = 0; h < HN; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const bool page = (flags >> (h0 + h) & 1) != 0;
-          const int key = tile * TILE + (h0 + h) * GRANULE + g + 8 * r;
-          bool any = false, every = true;
+          const bool page = (flags >> h & 1) != 0;
+          const int key = tile * TILE + h * GRANULE + g + 8 * r;
+          bool any = false, seen[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const bool seen = page && key < limit[nt][c];
-              any = any || seen;
-              every = every && seen;
-              if (!seen) sc[h][nt][2 * r + c] = -INFINITY;
+              seen[nt][c] = page && key < limit[nt][c];
+              any = any || seen[nt][c];
+              if (!seen[nt][c]) sc[h][nt][2 * r + c] = -INFINITY;
             }
-          if (!any) vs[h][r] = vm[h][r] = 0.f;
-          careful = careful || (any && !every && !(fabsf(vs[h][r]) + fabsf(vm[h][r]) < INFINITY));
+          if (!any) {
+            vs[h][r] = vm[h][r] = 0.f;
+          } else if (!(fabsf(vs[h][r]) + fabsf(vm[h][r]) < INFINITY)) {
+            // parameters that are no numbers must not meet the weight 0 of a column that does not see the key: the
+            // columns that see it take the NaN through their sum
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                if (seen[nt][c]) l[nt][c] = NAN;
+            vs[h][r] = vm[h][r] = 0.f;
+          }
         }
-      careful = __any_sync(0xffffffffu, careful);
     }
-    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[HN - 1][0], vs[HN - 1][1]));
+    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
     float top[NT][2];
     bool move = vmax > v_limit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[HN - 1][nt][c], sc[HN - 1][nt][2 + c]));
+        top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
         move = move || top[nt][c] > over[nt][c];
       }
     if (__any_sync(0xffffffffu, move)) {
@@ -678,7 +758,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             acc[nt][i][2 + c] *= both;
           }
 #pragma unroll
-          for (int h = 0; h < HN; ++h) {
+          for (int h = 0; h < 2; ++h) {
             sc[h][nt][c] -= rise;
             sc[h][nt][2 + c] -= rise;
           }
@@ -686,7 +766,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     }
     // ---- P^T, then O^T += V^T P^T
 #pragma unroll
-    for (int h = 0; h < HN; ++h) {
+    for (int h = 0; h < 2; ++h) {
       uint32_t pf[NT][2];
       const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * v_scale};
 #pragma unroll
@@ -698,21 +778,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
           const float pr = ex2f(sc[h][nt][k]);
           l[nt][c] += pr;
           w[k] = pr * vsn[r];
-          if (!careful) pm[nt][c] = fmaf(pr, vm[h][r], pm[nt][c]);
-        }
-        if (careful) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool seen = sc[h][nt][k] != -INFINITY;
-            pm[nt][k & 1] += seen ? ex2f(sc[h][nt][k]) * vm[h][k >> 1] : 0.0f;
-            if (!seen) w[k] = 0.0f;
-          }
+          pm[nt][c] = fmaf(pr, vm[h][r], pm[nt][c]);
         }
         const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
         pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
       }
-      const uint32_t st_addr = smem_u32(st) + (h0 + h) * GRANULE_BYTES;
+      const uint32_t st_addr = smem_u32(st) + h * GRANULE_BYTES;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t v[4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
@@ -728,7 +800,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         }
       }
     }
-    }
     __syncwarp();  // every lane has read the stage
     const int next = n + STAGES;
     if (next < count) {
@@ -743,7 +814,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   }
   if (ok) {
     __syncwarp();
-    if (count > 0) flush();
+    if (count > 0) flush(true);
   } else {
     // a wait ran out: this warp's copies may still be on their way into shared memory
     const uint64_t t_stop = globaltimer_ns() + 2000000ull;
@@ -790,7 +861,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     if (j >= min(w.fresh, p.max_new) || row < 0 || row >= p.rows) continue;
     auto link = [&](int i) -> const float* {
       const int w = sm.order[max(ch.start, 0) + i];
-      return ch.start >= 0 && i == 0 ? reinterpret_cast<const float*>(sm.ring[w][0]) + local * PARTIAL_FLOATS : sm.head[w][local];
+      const bool in_ring = (ch.start >= 0 && i == 0) || sm.ends[w].head_in_ring != 0;
+      return (in_ring ? reinterpret_cast<const float*>(sm.ring[w][0]) : p.heads + (static_cast<size_t>(blockIdx.x) * WARPS + w) * COLS * PARTIAL_FLOATS) + local * PARTIAL_FLOATS;
     };
     float sum, joined;
     const float4 v = join_links(ch.links, link, lane, sum, joined);
@@ -857,6 +929,7 @@ namespace paged {
 // 8 warps. 16 read the cache once where 8 would read it twice; 8 or fewer columns have no use for the second set.
 constexpr int ATTN_MAX_CTAS = 160;
 constexpr int attn_columns(long long columns) { return columns <= 8 ? 8 : 16; }
+constexpr int attn_warps(int cols) { return cols == 8 ? 16 : 8; }
 constexpr size_t attn_counter_bytes() { return ATTN_MAX_CTAS * sizeof(int); }
 static_assert(attn_counter_bytes() == DF_ATTENTION_PAGED4_COUNTER_BYTES, "the public header's number");
 
@@ -890,7 +963,7 @@ extern "C" size_t df_attention_paged4_workspace_bytes(int requests, int q_heads,
   using namespace df::paged;
   if (requests <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new <= 0 || q_heads % kv_heads != 0) return 0;
   const int cols = attn_columns(static_cast<long long>(max_new) * (q_heads / kv_heads));
-  const size_t partial = static_cast<size_t>(ATTN_MAX_CTAS) * 2 * cols * PARTIAL_FLOATS * sizeof(float);
+  const size_t partial = static_cast<size_t>(ATTN_MAX_CTAS) * (2 + attn_warps(cols)) * cols * PARTIAL_FLOATS * sizeof(float);
   return attn_counter_bytes() + static_cast<size_t>(requests + 1) / 2 * 2 * sizeof(uint2) + partial;
 }
 
@@ -944,6 +1017,7 @@ extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const voi
   p.arrived = static_cast<int*>(workspace);
   p.prefix = reinterpret_cast<uint2*>(static_cast<uint8_t*>(workspace) + attn_counter_bytes());
   p.partial = reinterpret_cast<float*>(p.prefix + (requests + 1) / 2 * 2);
+  p.heads = p.partial + static_cast<size_t>(ATTN_MAX_CTAS) * 2 * cols * PARTIAL_FLOATS;
   p.ld_q = ld_q;
   p.ld_out = ld_out;
   p.rows = rows;
@@ -960,5 +1034,5 @@ extern "C" int df_attention_paged4_bf16(const void* q, long long ld_q, const voi
   p.timeout_ns = timeout_ns();
   p.status = reinterpret_cast<Status*>(dev_status);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cols == 8 ? launch_attention<1, 16, 2>(p, grid, s) : launch_attention<2, 12, 2>(p, grid, s);
+  return cols == 8 ? launch_attention<1, attn_warps(8), 2>(p, grid, s) : launch_attention<2, attn_warps(16), 2>(p, grid, s);
 }

@@ -1,20 +1,25 @@
 // Log probability of a given token, entropy and the most likely tokens of rows of logits, in one pass over them.
 //
-// With m the largest logit of a row, S = sum exp(x - m) and U = sum exp(x - m) (x - m):
-//   log p(t) = (x_t - m) - log S,      entropy = log S - U / S
-// Every thread keeps (m, S, U) of what it has seen, in fp32, relative to its own maximum; they are joined by
-// rescaling to the larger one. exp(-inf) (x - m) counts as 0, so forbidden tokens (-inf) take no part.
+// In powers of two, with y = (x - m) log2(e) for a reference m, the largest logit, S = sum 2^y, U = sum 2^y y:
+//   log2 p(t) = y_t - log2 S,      entropy (bits) = log2 S - U / S
+// Every thread keeps (m, S, U) of what it has seen, in fp32 (two logits an instruction), relative to its own maximum;
+// they are joined by moving to the larger reference. Logits at or below -1e37 are lifted to -1e37 on the way, so that
+// 2^y y is 0 and not a NaN for the forbidden ones (-inf, or the type's lowest value); a slice that has nothing else is
+// gone through again with subtractions. They are no candidates either: what is missing from the k largest at the end
+// is filled with them, the lower index first.
 //
 // The k largest: a key of 64 bits, the logit made sortable in the upper half and the complement of its index in
 // the lower, is unique, so equal logits come out with the lower index first. A block goes through its part of the
-// row in chunks of 8192 logits. The first chunk gives a threshold: the k-th largest of the 256 threads' maxima is
-// reached by at least k logits and by few more; logits above it are put into a list (their order does not matter,
-// the keys decide), and a list that gets long is cut to its k largest, which raises the threshold. A chunk that
-// brings more than the list can hold (logits that grow along the row, or a great many equal ones) is selected
-// exactly by bisection over the keys instead.
+// row in chunks of 8192 logits. The first chunk gives a threshold: with r = ceil(k / 8), the smallest of the eight
+// warps' r-th largest lane maxima is reached by at least k logits and by few more. Logits above the threshold are put
+// into a list (their order does not matter, the keys decide); a list that gets long is cut to its k largest, which
+// raises the threshold. A chunk that brings more than the list can hold (logits that grow along the row, or a great
+// many equal ones) is selected exactly by bisection over the keys instead.
 //
-// Bound: HBM, each logit is read once. A row is cut into slices when there are few rows, and a second launch joins
-// the slices (the same launch joins the shards of a vocabulary that is split over ranks).
+// Bound: HBM, each logit is read once; then the exponentials (16 a clock and SM). The next chunk is fetched while one
+// is worked on. When there are few rows, a row is cut into slices: up to eight are one thread-block cluster, whose
+// first CTA joins them through distributed shared memory; more of them (a very long row) leave records in the
+// workspace for a second launch, which also joins the shards of a vocabulary that is split over ranks.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -29,14 +34,18 @@ constexpr int PER_THREAD = 32;                       // logits of a chunk a thre
 constexpr int CHUNK = THREADS * PER_THREAD;
 constexpr int MAX_TOP = 32;
 constexpr int LIST = 512;                            // candidates of a block
+constexpr int CUT_AT = 128;                          // a list that is longer is cut to the k largest
 constexpr int MAX_SLICES = 64;
+constexpr int CLUSTER_SLICES = 8;
+constexpr int LONG_SLICE = 16;                       // chunks of a slice above which a row is cut into more than a cluster
 constexpr int TARGET_BLOCKS = 592;                   // four a SM of 148
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -1e37f;                     // (LOWEST - 2e38) log2(e) is still finite
 
 typedef unsigned long long u64;
 
 struct Stats {
-  float m, s, u, x;  // maximum, sum exp, sum exp * (x - m), the given token's logit (-inf: not here)
+  float m, s, u, x;  // reference logit (-inf: none so far), sum 2^y and sum 2^y y of y = (logit - m) log2(e), the given token's logit (-inf: not here)
 };
 
 struct Params {
@@ -50,6 +59,7 @@ struct Params {
   long long ld;
   int id_bytes, rows, vocab, vocab_start, top, slices, parts;
   int finish;                 // 1: the results, 0: one record of the parts
+  int cluster;                // whether the slices of a row are one cluster
   size_t part_bytes;
   const uint8_t* parts_in;
 };
@@ -66,15 +76,43 @@ __device__ __forceinline__ uint32_t sortable(float x) {
 __device__ __forceinline__ float from_sortable(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) != 0u ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ u64 make_key(float x, uint32_t index) { return (static_cast<u64>(sortable(x)) << 32) | (0xffffffffu - index); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(u64 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 __device__ __forceinline__ void join(Stats& a, const Stats& b) {
   const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) {  // neither has a distribution; NaN sums stay
+  if (m == -INFINITY) {  // neither has a logit; NaN sums stay
     a.s += b.s;
     a.u += b.u;
   } else {
-    const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f);
-    const float fa = ex2f(da * LOG2E), fb = ex2f(db * LOG2E);
-    a.u = fa * (a.u + da * a.s) + fb * (b.u + db * b.s);
+    const float da = fmaxf((a.m - m) * LOG2E, -1e30f), db = fmaxf((b.m - m) * LOG2E, -1e30f);
+    const float fa = ex2f(da), fb = ex2f(db);
+    a.u = fa * fmaf(da, a.s, a.u) + fb * fmaf(db, b.s, b.u);
     a.s = fa * a.s + fb * b.s;
   }
   a.m = m;
@@ -93,26 +131,22 @@ __device__ __forceinline__ Stats shuffle(const Stats& v, int o) {
 struct Shared {
   u64 list[LIST];
   u64 kept[MAX_TOP];
-  uint32_t thread_max[THREADS];
+  uint32_t warp_value[THREADS / 32];
   Stats stats[THREADS / 32];
+  alignas(8) Stats total;
   int count, sum[2];
   uint32_t threshold;
 };
 
-// The sortable value that exactly `k` or more of the 256 thread maxima reach and k - 1 or fewer exceed (by the first warp).
-__device__ __forceinline__ uint32_t kth_of_threads(const uint32_t* v, int k, int lane) {
-  uint32_t x[THREADS / 32];
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) x[i] = v[i * 32 + lane];
-  uint32_t found = 0u;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t mid = found | (1u << bit);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) n += x[i] >= mid ? 1 : 0;
-    if (__reduce_add_sync(0xffffffffu, n) >= k) found = mid;
+// The r-th largest of the lanes' values (equal ones count as often as they occur).
+__device__ __forceinline__ uint32_t rth_of_lanes(uint32_t v, int r, int lane) {
+  uint32_t top = 0u;
+  for (int i = 0; i < r; ++i) {
+    top = __reduce_max_sync(0xffffffffu, v);
+    const unsigned at = __ballot_sync(0xffffffffu, v == top);
+    if (lane == __ffs(at) - 1) v = 0u;
   }
-  return found;
+  return top;
 }
 
 // Keeps the `top` largest of the list, largest first, in sm.kept (0: fewer than that). All threads; ends with a barrier.
@@ -133,40 +167,66 @@ struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
+  static constexpr uint32_t FORBIDDEN = 0xff80ff80u;  // -inf, twice
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ uint32_t raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint16_t*>(p); }
+  static __device__ __forceinline__ float get(const uint4& v, int j) {
+    const uint32_t w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
+    return __uint_as_float((j & 1) != 0 ? w & 0xffff0000u : w << 16);
+  }
+  static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) {
+    uint32_t& w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
+    w = (j & 1) != 0 ? (w & 0xffffu) | bits << 16 : (w & 0xffff0000u) | bits;
+  }
+  // largest of the vector's logits (NaN does not count)
+  static __device__ __forceinline__ float highest(const uint4& v) {
+    const __nv_bfloat162 a = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.x), reinterpret_cast<const __nv_bfloat162&>(v.y));
+    const __nv_bfloat162 b = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.z), reinterpret_cast<const __nv_bfloat162&>(v.w));
+    const __nv_bfloat162 m = __hmax2(a, b);
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  // pair i of the vector, no lower than LOWEST (NaN stays)
+  static __device__ __forceinline__ u64 pair(const uint4& v, int i) {
+    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    const __nv_bfloat162 low = __float2bfloat162_rn(LOWEST);
+    const __nv_bfloat162 h = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(w), low);
+    const uint32_t c = reinterpret_cast<const uint32_t&>(h);
+    return pack2(__uint_as_float(c << 16), __uint_as_float(c & 0xffff0000u));
+  }
 };
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
-    x[0] = __uint_as_float(v.x);
-    x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z);
-    x[3] = __uint_as_float(v.w);
-  }
+  static constexpr uint32_t FORBIDDEN = 0xff800000u;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ uint32_t raw(const float* p) { return __float_as_uint(*p); }
+  static __device__ __forceinline__ float get(const uint4& v, int j) { return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w); }
+  static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) { (j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w) = bits; }
+  static __device__ __forceinline__ float highest(const uint4& v) { return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3))); }
+  static __device__ __forceinline__ float lift(float x) {  // max that keeps NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(LOWEST));
+    return r;
+  }
+  static __device__ __forceinline__ u64 pair(const uint4& v, int i) { return pack2(lift(get(v, 2 * i)), lift(get(v, 2 * i + 1))); }
 };
 
+// From base 2 with the fp32 constant LOG2E, whose powers are those of e to 2^-26 of the exponent.
+__device__ __forceinline__ float to_nats(double bits) { return static_cast<float>(bits / static_cast<double>(LOG2E)); }
+__device__ __forceinline__ float logprob_of(float x, const Stats& s, float log_s) {
+  return to_nats((static_cast<double>(x) - static_cast<double>(s.m)) * static_cast<double>(LOG2E) - static_cast<double>(log_s));
+}
 __device__ __forceinline__ void write_results(const Params& p, int row, const Stats& s, const u64* kept) {
   const bool empty = s.m == -INFINITY && s.s == 0.0f;  // no token is allowed: no distribution
-  const float log_s = logf(s.s);
+  const float log_s = log2f(s.s);
   if (threadIdx.x == 0) {
-    p.logprob[row] = empty ? -INFINITY : (s.x - s.m) - log_s;
-    p.entropy[row] = empty ? 0.0f : log_s - s.u / s.s;
+    p.logprob[row] = empty ? -INFINITY : logprob_of(s.x, s, log_s);
+    p.entropy[row] = empty ? 0.0f : to_nats(static_cast<double>(log_s) - static_cast<double>(s.u / s.s));
   }
   if (static_cast<int>(threadIdx.x) < p.top) {
     const u64 key = kept[threadIdx.x];
     p.top_ids[static_cast<size_t>(row) * p.top + threadIdx.x] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-    p.top_logprobs[static_cast<size_t>(row) * p.top + threadIdx.x] =
-        empty ? -INFINITY : (from_sortable(static_cast<uint32_t>(key >> 32)) - s.m) - log_s;
+    p.top_logprobs[static_cast<size_t>(row) * p.top + threadIdx.x] = empty ? -INFINITY : logprob_of(from_sortable(static_cast<uint32_t>(key >> 32)), s, log_s);
   }
 }
 
@@ -177,8 +237,108 @@ __device__ __forceinline__ void write_record(const Params& p, int part, int row,
     reinterpret_cast<u64*>(base + static_cast<size_t>(p.rows) * sizeof(Stats))[static_cast<size_t>(row) * p.top + threadIdx.x] = kept[threadIdx.x];
 }
 
+// A chunk of this thread's logits, 16-byte vectors; what lies outside the row is -inf.
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const Params p) {
+__device__ __forceinline__ void load_chunk(uint4 (&v)[PER_THREAD / Vec<T>::N], const T* x0, int first, int lead, int vocab) {
+  constexpr int N = Vec<T>::N;
+#pragma unroll
+  for (int i = 0; i < PER_THREAD / N; ++i) {
+    const int e = (first + i * THREADS) * N - lead;  // first element of the vector
+    if (e >= 0 && e + N <= vocab) {
+      v[i] = __ldg(reinterpret_cast<const uint4*>(x0 + e));
+    } else {
+      v[i] = make_uint4(Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (e + j >= 0 && e + j < vocab) Vec<T>::put(v[i], j, Vec<T>::raw(x0 + e + j));
+    }
+  }
+}
+
+// A chunk (elements [e0, e1) of the row) with more candidates than the list holds: the `top` largest keys of it and of
+// what the list held before it, exactly, by bisection. They replace the list; returns the smallest one's value. (Reads
+// the chunk again: rows of equal or of rising logits come here, others do not.) All threads.
+template <typename T>
+__device__ __noinline__ uint32_t select_exactly(Shared& sm, const T* x0, int e0, int e1, int top) {
+  const int tid = threadIdx.x;
+  // the list is full; its entries of this chunk are in the chunk too: only those with an index before it count
+  auto older = [&](u64 key) { return 0xffffffffu - static_cast<uint32_t>(key) < static_cast<uint32_t>(e0); };
+  u64 found = 0ull;
+  for (int bit = 63; bit >= 0; --bit) {
+    const u64 mid = found | (1ull << bit);
+    int n = 0;
+    for (int e = e0 + tid; e < e1; e += THREADS) n += make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e)) >= mid ? 1 : 0;
+    for (int i = tid; i < LIST; i += THREADS) n += sm.list[i] >= mid && older(sm.list[i]) ? 1 : 0;
+    if (tid == 0) sm.sum[bit & 1] = 0;
+    __syncthreads();
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0) atomicAdd(&sm.sum[bit & 1], n);
+    __syncthreads();
+    if (sm.sum[bit & 1] >= top) found = mid;
+  }
+  if (tid == 0) sm.count = 0;
+  __syncthreads();
+  for (int i = tid; i < LIST; i += THREADS)
+    if (sm.list[i] >= found && older(sm.list[i])) sm.kept[atomicAdd(&sm.count, 1)] = sm.list[i];
+  for (int e = e0 + tid; e < e1; e += THREADS) {
+    const u64 key = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
+    if (key >= found) sm.kept[atomicAdd(&sm.count, 1)] = key;
+  }
+  __syncthreads();
+  return static_cast<uint32_t>(found >> 32);
+}
+
+// The list has fewer than `top` keys because the other logits of elements [e0, e1) are forbidden (at or below LOWEST):
+// adds those, larger values first, of equal ones the lower index. All threads.
+template <typename T>
+__device__ __noinline__ void fill_forbidden(Shared& sm, const T* x0, int e0, int e1, int top) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t below = sortable(LOWEST) + 1u;  // values under it are still to be added
+  while (true) {
+    uint32_t value = 0u;                   // the largest of them; 0: none is left
+    for (int e = e0 + tid; e < e1; e += THREADS) {
+      const uint32_t o = sortable(Vec<T>::one(x0 + e));
+      if (o < below) value = max(value, o);
+    }
+    __syncthreads();
+    value = __reduce_max_sync(0xffffffffu, value);
+    if (lane == 0) sm.warp_value[warp] = value;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) value = max(value, sm.warp_value[i]);
+    int count = sm.count;
+    if (value == 0u || count >= top) return;
+    for (int e = e0; e < e1 && count < top; e += THREADS) {  // in order of the index
+      const bool here = e + tid < e1 && sortable(Vec<T>::one(x0 + e + tid)) == value;
+      const unsigned votes = __ballot_sync(0xffffffffu, here);
+      __syncthreads();
+      if (lane == 0) sm.warp_value[warp] = __popc(votes);
+      __syncthreads();
+      int before = 0, all = 0;
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) {
+        if (i < warp) before += sm.warp_value[i];
+        all += sm.warp_value[i];
+      }
+      const int at = count + before + __popc(votes & ((1u << lane) - 1u));
+      if (here && at < top) sm.list[at] = static_cast<u64>(value) << 32 | (0xffffffffu - static_cast<uint32_t>(e + tid));
+      count = min(count + all, top);
+    }
+    __syncthreads();
+    if (tid == 0) sm.count = count;
+    __syncthreads();
+    below = value;
+  }
+}
+
+__device__ __forceinline__ u64 read_remote(const u64* p, unsigned rank) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprobs_kernel(const Params p) {
   constexpr int N = Vec<T>::N, VECS = PER_THREAD / N;
   __shared__ Shared sm;
   grid_dependency_wait();
@@ -191,131 +351,189 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const Params
   const int vectors = (p.vocab + lead + N - 1) / N;
   const int chunks = (vectors + THREADS * VECS - 1) / (THREADS * VECS);
   const int c0 = static_cast<int>(static_cast<long long>(chunks) * slice / p.slices), c1 = static_cast<int>(static_cast<long long>(chunks) * (slice + 1) / p.slices);
-  if (tid == 0) {
-    sm.count = 0;
-    sm.threshold = 0u;
+  float given = -INFINITY;
+  if (slice == 0 && tid == 0) {
+    const long long id = (p.id_bytes == 8 ? static_cast<const long long*>(p.ids)[row] : static_cast<const int*>(p.ids)[row]) - p.vocab_start;
+    if (id >= 0 && id < p.vocab) given = Vec<T>::one(x0 + id);
   }
-  if (tid < MAX_TOP) sm.kept[tid] = 0ull;
-  Stats st{-INFINITY, 0.0f, 0.0f, -INFINITY};
-  bool first = true;
-  for (int c = c0; c < c1; ++c) {
-    float x[PER_THREAD];
-    const int v0 = c * THREADS * VECS + tid;
+  if (TOP && tid == 0) sm.count = 0;
+  float high = -INFINITY;                 // largest logit of this thread
+  u64 s2 = pack2(0.f, 0.f), u2 = s2;
+  uint32_t above = 0u;                    // sortable value that a logit has to exceed to be a candidate
+  const uint32_t lowest = sortable(LOWEST);
+  const u64 scale = pack2(LOG2E, LOG2E);
+  uint4 v[VECS];
+  if (c0 < c1) load_chunk<T>(v, x0, c0 * THREADS * VECS + tid, lead, p.vocab);
+  for (int ch = c0; ch < c1; ++ch) {
+    uint4 ahead[VECS];
+    const int first = ch * THREADS * VECS + tid;
+    if (ch + 1 < c1) load_chunk<T>(ahead, x0, first + THREADS * VECS, lead, p.vocab);
+    float high_of[VECS], now = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int e = (v0 + i * THREADS) * N - lead;  // first element of the vector
-      if (e >= 0 && e + N <= p.vocab) {
-        Vec<T>::unpack(*reinterpret_cast<const uint4*>(x0 + e), x + i * N);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[i * N + j] = e + j >= 0 && e + j < p.vocab ? Vec<T>::one(x0 + e + j) : -INFINITY;
-      }
+      high_of[i] = Vec<T>::highest(v[i]);
+      now = fmaxf(now, high_of[i]);
     }
-    float high = x[0];
-#pragma unroll
-    for (int i = 1; i < PER_THREAD; ++i) high = fmaxf(high, x[i]);
     // ---- sums
-    if (high > st.m) {
-      if (st.m != -INFINITY) {
-        const float d = st.m - high, f = ex2f(d * LOG2E);
-        st.u = f * (st.u + d * st.s);
-        st.s *= f;
+    if (now > high) {
+      if (high > LOWEST) {
+        const float d = (high - now) * LOG2E, f = ex2f(d);
+        const float2 s = unpack2(s2), u = unpack2(u2);
+        s2 = pack2(f * s.x, f * s.y);
+        u2 = pack2(f * fmaf(d, s.x, u.x), f * fmaf(d, s.y, u.y));
       }
-      st.m = high;
+      high = now;
     }
-    const float ref = st.m == -INFINITY ? 0.0f : st.m;
+    const float ref = high > LOWEST ? high : 0.0f;  // without a reference 2^(LOWEST) is 0, too
+    const u64 minus = pack2(-ref, -ref);
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) {
-      const float d = x[i] - ref, e = ex2f(d * LOG2E);
-      st.s += e;
-      st.u = fmaf(e, fmaxf(d, -1e30f), st.u);
-    }
+    for (int i = 0; i < VECS; ++i)
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        const u64 y = mul2(add2(Vec<T>::pair(v[i], j), minus), scale);
+        const float2 yy = unpack2(y);
+        const u64 e = pack2(ex2f(yy.x), ex2f(yy.y));
+        s2 = add2(s2, e);
+        u2 = fma2(e, y, u2);
+      }
     // ---- candidates
-    if (p.top > 0) {
-      auto index_of = [&](int i) { return (v0 + (i / N) * THREADS) * N - lead + i % N; };
-      auto valid = [&](int i) { const int e = index_of(i); return e >= 0 && e < p.vocab; };
-      if (first) {
-        sm.thread_max[tid] = sortable(high);
+    if (TOP) {
+      if (ch == c0) {
+        const uint32_t r = rth_of_lanes(sortable(now), (p.top + THREADS / 32 - 1) / (THREADS / 32), lane);
+        if (lane == 0) sm.warp_value[warp] = r;
         __syncthreads();
-        if (warp == 0) {
-          const uint32_t t = kth_of_threads(sm.thread_max, p.top, lane);
-          if (lane == 0) sm.threshold = t - 1u;  // the first chunk takes what reaches it
-        }
-        __syncthreads();
-      }
-      const uint32_t above = sm.threshold;
-      const int before = sm.count;
-      __syncthreads();
-      if (sortable(high) > above) {
+        above = sm.warp_value[0];
 #pragma unroll
-        for (int i = 0; i < PER_THREAD; ++i)
-          if (sortable(x[i]) > above && valid(i)) {
-            const int at = atomicAdd(&sm.count, 1);
-            if (at < LIST) sm.list[at] = make_key(x[i], static_cast<uint32_t>(index_of(i)));
+        for (int i = 1; i < THREADS / 32; ++i) above = min(above, sm.warp_value[i]);
+      }
+      // the first chunk takes what reaches its threshold; later logits have higher indices: those equal to it lose
+      const uint32_t past = max(ch == c0 ? above - 1u : above, lowest);
+      bool many = false;
+      if (sortable(now) > past) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+          if (sortable(high_of[i]) > past) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const float x = Vec<T>::get(v[i], j);
+              if (sortable(x) > past) {
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < LIST) sm.list[at] = make_key(x, static_cast<uint32_t>((first + i * THREADS) * N - lead + j));
+                many = many || at >= CUT_AT;
+              }
+            }
           }
       }
-      __syncthreads();
-      const int count = sm.count;
-      if (count > LIST) {
-        // too many: the k-th largest key of the list so far and this chunk by bisection, then exactly those that reach it
-        u64 found = 0ull;
-        for (int bit = 63; bit >= 0; --bit) {
-          const u64 mid = found | (1ull << bit);
-          int n = 0;
-#pragma unroll
-          for (int i = 0; i < PER_THREAD; ++i) n += valid(i) && make_key(x[i], static_cast<uint32_t>(index_of(i))) >= mid ? 1 : 0;
-          for (int i = tid; i < before; i += THREADS) n += sm.list[i] >= mid ? 1 : 0;
-          if (tid == 0) sm.sum[bit & 1] = 0;
-          __syncthreads();
-          n = __reduce_add_sync(0xffffffffu, n);
-          if (lane == 0) atomicAdd(&sm.sum[bit & 1], n);
-          __syncthreads();
-          if (sm.sum[bit & 1] >= p.top) found = mid;
+      if (__syncthreads_or(many)) {
+        const int count = sm.count;
+        if (count > LIST) {
+          above = select_exactly(sm, x0, max(ch * THREADS * VECS * N - lead, 0), min((ch + 1) * THREADS * VECS * N - lead, p.vocab), p.top);
+        } else {
+          keep_largest(sm, count, p.top);
+          above = max(above, static_cast<uint32_t>(sm.kept[p.top - 1] >> 32));
         }
-        if (tid == 0) sm.count = 0;
-        __syncthreads();
-        for (int i = tid; i < before; i += THREADS)
-          if (sm.list[i] >= found) sm.kept[atomicAdd(&sm.count, 1)] = sm.list[i];
-#pragma unroll
-        for (int i = 0; i < PER_THREAD; ++i) {
-          const u64 key = make_key(x[i], static_cast<uint32_t>(index_of(i)));
-          if (valid(i) && key >= found) sm.kept[atomicAdd(&sm.count, 1)] = key;
-        }
-        __syncthreads();
         if (tid < p.top) sm.list[tid] = sm.kept[tid];
-        if (tid == 0) sm.threshold = static_cast<uint32_t>(found >> 32);
-      } else if (count > LIST / 2) {
-        keep_largest(sm, count, p.top);
-        if (tid < p.top) sm.list[tid] = sm.kept[tid];
-        if (tid == 0) {
-          sm.count = p.top;
-          sm.threshold = static_cast<uint32_t>(sm.kept[p.top - 1] >> 32);
-        }
-      } else if (first && tid == 0 && count >= p.top) {
-        sm.threshold = above + 1u;  // later logits have higher indices: those equal to it lose
+        if (tid == 0) sm.count = p.top;
+        __syncthreads();
       }
-      __syncthreads();
-      first = false;
     }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) v[i] = ahead[i];
   }
   // ---- the block's sums
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) join(st, shuffle(st, o));
-  if (lane == 0) sm.stats[warp] = st;
-  __syncthreads();
-  st = sm.stats[0];
-#pragma unroll
-  for (int w = 1; w < THREADS / 32; ++w) join(st, sm.stats[w]);
-  if (slice == 0) {
-    const long long id = (p.id_bytes == 8 ? static_cast<const long long*>(p.ids)[row] : static_cast<const int*>(p.ids)[row]) - p.vocab_start;
-    if (id >= 0 && id < p.vocab) st.x = Vec<T>::one(x0 + id);
+  const float2 s = unpack2(s2), u = unpack2(u2);
+  Stats st{-INFINITY, 0.0f, 0.0f, given};
+  if (high > LOWEST) {
+    st.m = high;
+    st.s = s.x + s.y;
+    st.u = u.x + u.y;
+  } else if (s.x + s.y != s.x + s.y) {
+    st.s = NAN;  // a NaN among forbidden tokens
   }
-  if (p.top > 0) keep_largest(sm, min(sm.count, LIST), p.top);
-  if (p.vocab_start != 0 && static_cast<int>(threadIdx.x) < p.top && sm.kept[tid] != 0ull) sm.kept[tid] -= static_cast<u64>(p.vocab_start);
-  if (p.finish && p.slices == 1)
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    join(st, shuffle(st, o));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  }
+  if (lane == 0) {
+    sm.stats[warp] = st;
+    sm.warp_value[warp] = __float_as_uint(high);
+  }
+  __syncthreads();
+  const int e0 = max(c0 * THREADS * VECS * N - lead, 0), e1 = min(c1 * THREADS * VECS * N - lead, p.vocab);
+  if (warp == 0) {
+    st = sm.stats[lane & 7];
+    high = __uint_as_float(sm.warp_value[lane & 7]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      join(st, shuffle(st, o));
+      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    if (high <= LOWEST) {
+      // nothing above LOWEST: forbidden tokens only, or finite logits that low, which are summed with subtractions
+      const bool nan = st.s != st.s;
+      float sum = 0.0f, moment = 0.0f;
+      if (high > -INFINITY)
+        for (int e = e0 + lane; e < e1; e += 32) {
+          const float y = (Vec<T>::one(x0 + e) - high) * LOG2E, w = ex2f(y);
+          sum += w;
+          if (w > 0.0f) moment = fmaf(w, y, moment);
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        moment += __shfl_xor_sync(0xffffffffu, moment, o);
+      }
+      st.m = high;
+      st.s = nan ? NAN : sum;
+      st.u = moment;
+    }
+    if (lane == 0) sm.total = st;
+  }
+  if (TOP) {
+    if (sm.count < p.top) fill_forbidden(sm, x0, e0, e1, p.top);
+    keep_largest(sm, min(sm.count, LIST), p.top);
+  } else {
+    __syncthreads();
+  }
+  if (TOP && p.vocab_start != 0 && tid < p.top && sm.kept[tid] != 0ull) sm.kept[tid] -= static_cast<u64>(p.vocab_start);
+  if (p.cluster) {
+    cluster_sync();  // every slice's sums and keys are in its shared memory
+    if (slice == 0) {
+      if (warp == 0) {
+        st = sm.total;
+        if (lane < p.slices) {
+          const u64 a = read_remote(reinterpret_cast<const u64*>(&sm.total), lane), b = read_remote(reinterpret_cast<const u64*>(&sm.total) + 1, lane);
+          const float2 ms = unpack2(a), ux = unpack2(b);
+          st = Stats{ms.x, ms.y, ux.x, ux.y};
+        } else {
+          st = Stats{-INFINITY, 0.0f, 0.0f, -INFINITY};
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) join(st, shuffle(st, o));
+        __syncwarp();
+        if (lane == 0) sm.stats[0] = st;
+      }
+      if (TOP) {
+        const int n = p.slices * p.top;  // at most 8 * 32, a key a thread
+        const u64 key = tid < n ? read_remote(&sm.kept[tid % p.top], tid / p.top) : 0ull;
+        if (tid < n) sm.list[tid] = key;
+        __syncthreads();
+        keep_largest(sm, n, p.top);
+      } else {
+        __syncthreads();
+      }
+      st = sm.stats[0];
+    }
+    cluster_sync();  // nobody leaves while its shared memory is read
+    if (slice != 0) return;
+  } else {
+    st = sm.total;
+  }
+  if (p.finish && (p.cluster || p.slices == 1))
     write_results(p, row, st, sm.kept);
   else
-    write_record(p, slice, row, st, sm.kept);
+    write_record(p, p.cluster ? 0 : slice, row, st, sm.kept);
 }
 
 // Joins the parts of a row: sums in the order of the parts, the k largest of their keys.
@@ -347,25 +565,36 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const Para
     write_record(p, 0, row, st, kept);
 }
 
-// Slices a row is cut into: enough blocks to fill the device, no slice shorter than a chunk.
+// Slices a row is cut into: enough blocks to fill the device and no slice shorter than a chunk, at most a cluster of
+// them unless that leaves long slices to few rows.
 int slices_of(int rows, int vocab) {
   const int chunks = (vocab + CHUNK - 1) / CHUNK;
-  int s = (TARGET_BLOCKS + rows - 1) / rows;
-  if (s > chunks) s = chunks;
-  return s < 1 ? 1 : (s > MAX_SLICES ? MAX_SLICES : s);
+  int want = (TARGET_BLOCKS + rows - 1) / rows;
+  if (want > chunks) want = chunks;
+  if (want > CLUSTER_SLICES && (chunks + CLUSTER_SLICES - 1) / CLUSTER_SLICES > LONG_SLICE) return want < MAX_SLICES ? want : MAX_SLICES;
+  int s = 1;
+  while (s < CLUSTER_SLICES && 2 * s <= want) s *= 2;
+  return s;
 }
 size_t record_bytes(int rows, int top) { return static_cast<size_t>(rows) * (sizeof(Stats) + static_cast<size_t>(top) * sizeof(u64)); }
 
 template <typename Kernel>
-int launch(Kernel kernel, unsigned blocks, size_t smem, const Params& p, void* stream) {
+int launch(Kernel kernel, unsigned blocks, unsigned cluster, size_t smem, const Params& p, void* stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr;
-  cfg.numAttrs = dependent_launch_attr(&attr);
-  cfg.attrs = &attr;
+  cudaLaunchAttribute attrs[2];
+  cfg.attrs = attrs;
+  cfg.numAttrs = dependent_launch_attr(&attrs[0]);
+  if (cluster > 1) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = cluster;
+    attrs[cfg.numAttrs].val.clusterDim.y = 1;
+    attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -398,28 +627,32 @@ extern "C" size_t df_token_logprobs_record_bytes(int rows, int top) {
 extern "C" size_t df_token_logprobs_workspace_bytes(int rows, int vocab, int top) {
   using namespace df::logprobs;
   if (rows <= 0 || vocab <= 0 || top < 0 || top > MAX_TOP) return 0;
-  return static_cast<size_t>(slices_of(rows, vocab)) * record_bytes(rows, top);
+  const int slices = slices_of(rows, vocab);
+  return slices > CLUSTER_SLICES ? slices * record_bytes(rows, top) : 16;  // a cluster needs none
 }
 
 static int run_logprobs(df::logprobs::Params& p, int fp32, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace df;
   using namespace df::logprobs;
   p.slices = slices_of(p.rows, p.vocab);
+  p.cluster = p.slices > 1 && p.slices <= CLUSTER_SLICES;
   p.part_bytes = record_bytes(p.rows, p.top);
   uint8_t* result = p.record;
-  if (p.slices > 1) {
+  if (p.slices > CLUSTER_SLICES) {
     const size_t need = p.slices * p.part_bytes;
     if (workspace == nullptr || workspace_bytes < need) return fail(DF_EINVAL, "workspace of %zu bytes is too small (need %zu)", workspace_bytes, need);
     if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(DF_EINVAL, "the workspace must be 16-byte aligned");
     p.record = static_cast<uint8_t*>(workspace);
   }
-  const unsigned blocks = static_cast<unsigned>(p.rows) * static_cast<unsigned>(p.slices);
-  int rc = fp32 ? launch(token_logprobs_kernel<float>, blocks, 0, p, stream) : launch(token_logprobs_kernel<__nv_bfloat16>, blocks, 0, p, stream);
-  if (rc != DF_OK || p.slices == 1) return rc;
+  const unsigned blocks = static_cast<unsigned>(p.rows) * static_cast<unsigned>(p.slices), cluster = p.cluster ? p.slices : 1;
+  auto kernel = fp32 ? (p.top > 0 ? token_logprobs_kernel<float, true> : token_logprobs_kernel<float, false>)
+                     : (p.top > 0 ? token_logprobs_kernel<__nv_bfloat16, true> : token_logprobs_kernel<__nv_bfloat16, false>);
+  const int rc = launch(kernel, blocks, cluster, 0, p, stream);
+  if (rc != DF_OK || p.slices <= CLUSTER_SLICES) return rc;
   p.parts = p.slices;
   p.parts_in = static_cast<const uint8_t*>(workspace);
   p.record = result;
-  return launch(token_logprobs_join_kernel, static_cast<unsigned>(p.rows), static_cast<size_t>(p.parts) * p.top * sizeof(u64), p, stream);
+  return launch(token_logprobs_join_kernel, static_cast<unsigned>(p.rows), 1, static_cast<size_t>(p.parts) * p.top * sizeof(u64), p, stream);
 }
 
 extern "C" int df_token_logprobs(const void* logits, int fp32, long long ld, const void* ids_dev, int id_bytes, int rows, int vocab,
@@ -489,5 +722,5 @@ extern "C" int df_token_logprobs_join(const void* records_dev, int parts, int ro
   p.entropy = entropy_dev;
   p.top_ids = top_ids_dev;
   p.top_logprobs = top_logprobs_dev;
-  return launch(token_logprobs_join_kernel, static_cast<unsigned>(rows), static_cast<size_t>(parts) * top * sizeof(u64), p, stream);
+  return launch(token_logprobs_join_kernel, static_cast<unsigned>(rows), 1, static_cast<size_t>(parts) * top * sizeof(u64), p, stream);
 }

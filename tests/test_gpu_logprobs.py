@@ -97,13 +97,39 @@ def test_forbidden_tokens(ops, allowed):
         _check(_run(ops, y.cuda(), ids, top), y, ids, top)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masks_of_the_lowest_value(ops, dtype):
+    """Forbidden by the type's lowest value instead of -inf; both kinds; a row of nothing but lowest values is uniform."""
+    vocab, top = 20000, 12
+    low = torch.finfo(dtype).min
+    x = torch.full((4, vocab), low, dtype=torch.float64)
+    x[0, [5, 19000, 700]] = torch.tensor([1.0, 2.0, 0.5], dtype=torch.float64)
+    x[1, 3:] = -math.inf
+    x[1, [100, 9000]] = torch.tensor([-3.0, 4.0], dtype=torch.float64)
+    x[3, ::2] = -math.inf
+    x = x.to(dtype)
+    ids = [700, 9000, 123, 1]
+    _check(_run(ops, x.cuda(), ids, top), x, ids, top)
+
+
+def test_a_very_long_row(ops):
+    """So long that a row is cut into more slices than a cluster has; the slices' records go through the workspace."""
+    vocab = 1_300_000
+    x = (torch.randn(1, vocab, generator=torch.Generator().manual_seed(12)) * 3).bfloat16()
+    assert ops.token_logprobs_workspace(1, vocab, 20).numel() > 1000
+    _check(_run(ops, x.cuda(), [vocab - 1], 20), x, [vocab - 1], 20)
+
+
 def test_nan_and_infinity_are_not_lost(ops):
-    x = torch.randn(3, 9000)
+    x = torch.randn(4, 9000)
     x[0, 4000] = float("nan")
     x[1, 8999] = math.inf
-    got = _run(ops, x.cuda(), [1, 2, 3], 2)
-    for t in (got[0], got[1]):
-        assert torch.isnan(t[:2]).all() and torch.isfinite(t[2]).all()
+    x[3] = -math.inf
+    x[3, 17] = float("nan")
+    for dtype in (torch.float32, torch.bfloat16):
+        got = _run(ops, x.to(dtype).cuda(), [1, 2, 3, 4], 2)
+        for t in (got[0], got[1]):
+            assert torch.isnan(t[[0, 1, 3]]).all() and torch.isfinite(t[2]).all()
 
 
 @pytest.mark.parametrize("scale", [1e-30, 50.0, 1e30])

@@ -173,7 +173,7 @@ def test_logprob_refusals(native_lib):
     _refused(native_lib, -3, "32", name, *call(top=33))
     _refused(native_lib, -3, "vocabulary", name, *call(vocab=4, top=5))
     _refused(native_lib, -1, "aligned", name, *call(logits=p + 1))
-    _refused(native_lib, -1, "too small", name, *call(vocab=100000, ld=100000, ws_bytes=8))
+    _refused(native_lib, -1, "too small", name, *call(rows=1, vocab=2000000, ld=2000000, ws_bytes=8))
     shard = "df_token_logprobs_shard"
     _refused(native_lib, -1, "vocab_start", shard, p, 0, 100, p, 8, 2, 100, -1, 5, p, p, 1 << 30, None)
     _refused(native_lib, -1, "NULL", shard, p, 0, 100, p, 8, 2, 100, 0, 5, None, p, 1 << 30, None)
