@@ -3,7 +3,7 @@
 // In powers of two, with y = (x - m) log2(e) for a reference m, the largest logit, S = sum 2^y, U = sum 2^y y:
 //   log2 p(t) = y_t - log2 S,      entropy (bits) = log2 S - U / S
 // Every thread keeps (m, S, U) of what it has seen, in fp32 (two logits an instruction), relative to its own maximum;
-// they are joined by moving to the larger reference. Logits at or below -1e37 are lifted to -1e37 on the way, so that
+// they are joined by moving to the larger reference. Logits at or below -2^123 are lifted to -2^123 on the way, so that
 // 2^y y is 0 and not a NaN for the forbidden ones (-inf, or the type's lowest value); a slice that has nothing else is
 // gone through again with subtractions. They are no candidates either: what is missing from the k largest at the end
 // is filled with them, the lower index first.
@@ -12,9 +12,10 @@
 // the lower, is unique, so equal logits come out with the lower index first. A block goes through its part of the
 // row in chunks of 8192 logits. The first chunk gives a threshold: with r = ceil(k / 8), the smallest of the eight
 // warps' r-th largest lane maxima is reached by at least k logits and by few more. Logits above the threshold are put
-// into a list (their order does not matter, the keys decide); a list that gets long is cut to its k largest, which
-// raises the threshold. A chunk that brings more than the list can hold (logits that grow along the row, or a great
-// many equal ones) is selected exactly by bisection over the keys instead.
+// into a list (their order does not matter, the keys decide). The block looks at the list after 1, 2, 4, 8, ... chunks
+// (as many as bring as many logits above the threshold again): a long one is thinned the same way, which raises the
+// threshold. Chunks that bring more than the list can hold (logits that grow along the row, or a great many equal
+// ones) are selected exactly by bisection over the keys instead.
 //
 // Bound: HBM, each logit is read once; then the exponentials (16 a clock and SM). The next chunk is fetched while one
 // is worked on. When there are few rows, a row is cut into slices: up to eight are one thread-block cluster, whose
@@ -34,13 +35,13 @@ constexpr int PER_THREAD = 32;                       // logits of a chunk a thre
 constexpr int CHUNK = THREADS * PER_THREAD;
 constexpr int MAX_TOP = 32;
 constexpr int LIST = 512;                            // candidates of a block
-constexpr int CUT_AT = 128;                          // a list that is longer is cut to the k largest
+constexpr int THIN_AT = 64;                          // a list that is longer is thinned
 constexpr int MAX_SLICES = 64;
 constexpr int CLUSTER_SLICES = 8;
 constexpr int LONG_SLICE = 16;                       // chunks of a slice above which a row is cut into more than a cluster
 constexpr int TARGET_BLOCKS = 592;                   // four a SM of 148
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LOWEST = -1e37f;                     // (LOWEST - 2e38) log2(e) is still finite
+constexpr float LOWEST = -0x1p123f;                  // a number of both types; (LOWEST - 2e38) log2(e) is still finite
 
 typedef unsigned long long u64;
 
@@ -149,6 +150,32 @@ __device__ __forceinline__ uint32_t rth_of_lanes(uint32_t v, int r, int lane) {
   return top;
 }
 
+// The largest number of the logits' type below t.
+__device__ __forceinline__ float just_below(float t, uint32_t ulp) {
+  const uint32_t b = __float_as_uint(t);
+  return __uint_as_float(t > 0.0f ? b - ulp : (t < 0.0f ? b + ulp : 0x80000000u | ulp));
+}
+
+// Leaves what reaches a threshold in the list: with r = ceil(top / 8) the smallest of the warps' r-th largest values,
+// which at least `top` keys reach. Returns its sortable value. `count` (more than THIN_AT, at most LIST) keys; all threads.
+__device__ __forceinline__ uint32_t thin(Shared& sm, int count, int top) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i0 = lane * (THREADS / 32) + warp, i1 = i0 + THREADS;  // every warp has its share of the keys
+  const u64 k0 = i0 < count ? sm.list[i0] : 0ull, k1 = i1 < count ? sm.list[i1] : 0ull;
+  const uint32_t v0 = static_cast<uint32_t>(k0 >> 32), v1 = static_cast<uint32_t>(k1 >> 32);
+  const uint32_t r = rth_of_lanes(max(v0, v1), (top + THREADS / 32 - 1) / (THREADS / 32), lane);
+  if (lane == 0) sm.warp_value[warp] = r;
+  if (threadIdx.x == 0) sm.count = 0;
+  __syncthreads();
+  uint32_t reach = sm.warp_value[0];
+#pragma unroll
+  for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
+  if (k0 != 0ull && v0 >= reach) sm.list[atomicAdd(&sm.count, 1)] = k0;
+  if (k1 != 0ull && v1 >= reach) sm.list[atomicAdd(&sm.count, 1)] = k1;
+  __syncthreads();
+  return reach;
+}
+
 // Keeps the `top` largest of the list, largest first, in sm.kept (0: fewer than that). All threads; ends with a barrier.
 __device__ __forceinline__ void keep_largest(Shared& sm, int count, int top) {
   if (threadIdx.x < MAX_TOP) sm.kept[threadIdx.x] = 0ull;
@@ -168,11 +195,16 @@ template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr uint32_t FORBIDDEN = 0xff80ff80u;  // -inf, twice
+  static constexpr uint32_t ULP = 0x10000u;           // of the fp32 bits of a logit
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ uint32_t raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint16_t*>(p); }
-  static __device__ __forceinline__ float get(const uint4& v, int j) {
-    const uint32_t w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
-    return __uint_as_float((j & 1) != 0 ? w & 0xffff0000u : w << 16);
+  // bit j of the result: whether logit j of the vector exceeds thr
+  static __device__ __forceinline__ uint32_t exceeding(const uint4& v, float thr) {
+    const __nv_bfloat162 t = __float2bfloat162_rn(thr);
+    const uint32_t a = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.x), t), b = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.y), t);
+    const uint32_t c = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.z), t), d = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.w), t);
+    const uint32_t m = (a & 0x00010001u) | (b & 0x00040004u) | (c & 0x00100010u) | (d & 0x00400040u);  // 2 i and 16 + 2 i
+    return (m | m >> 15) & 0xffu;
   }
   static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) {
     uint32_t& w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
@@ -198,9 +230,13 @@ template <>
 struct Vec<float> {
   static constexpr int N = 4;
   static constexpr uint32_t FORBIDDEN = 0xff800000u;
+  static constexpr uint32_t ULP = 1u;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ uint32_t raw(const float* p) { return __float_as_uint(*p); }
   static __device__ __forceinline__ float get(const uint4& v, int j) { return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w); }
+  static __device__ __forceinline__ uint32_t exceeding(const uint4& v, float thr) {
+    return (get(v, 0) > thr ? 1u : 0u) | (get(v, 1) > thr ? 2u : 0u) | (get(v, 2) > thr ? 4u : 0u) | (get(v, 3) > thr ? 8u : 0u);
+  }
   static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) { (j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w) = bits; }
   static __device__ __forceinline__ float highest(const uint4& v) { return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3))); }
   static __device__ __forceinline__ float lift(float x) {  // max that keeps NaN
@@ -359,8 +395,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
   if (TOP && tid == 0) sm.count = 0;
   float high = -INFINITY;                 // largest logit of this thread
   u64 s2 = pack2(0.f, 0.f), u2 = s2;
-  uint32_t above = 0u;                    // sortable value that a logit has to exceed to be a candidate
-  const uint32_t lowest = sortable(LOWEST);
+  float thr = LOWEST;                     // a candidate exceeds it
+  int look = c0, group = c0;              // the list is looked at after chunk `look`; first chunk since the last look
   const u64 scale = pack2(LOG2E, LOG2E);
   uint4 v[VECS];
   if (c0 < c1) load_chunk<T>(v, x0, c0 * THREADS * VECS + tid, lead, p.vocab);
@@ -398,43 +434,50 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
       }
     // ---- candidates
     if (TOP) {
+      float first_thr = LOWEST;
       if (ch == c0) {
         const uint32_t r = rth_of_lanes(sortable(now), (p.top + THREADS / 32 - 1) / (THREADS / 32), lane);
         if (lane == 0) sm.warp_value[warp] = r;
         __syncthreads();
-        above = sm.warp_value[0];
+        uint32_t reach = sm.warp_value[0];
 #pragma unroll
-        for (int i = 1; i < THREADS / 32; ++i) above = min(above, sm.warp_value[i]);
+        for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
+        // the first chunk takes what reaches this; later logits have higher indices: those equal to it lose
+        thr = fmaxf(from_sortable(reach), LOWEST);
+        if (thr > LOWEST) first_thr = just_below(thr, Vec<T>::ULP);
       }
-      // the first chunk takes what reaches its threshold; later logits have higher indices: those equal to it lose
-      const uint32_t past = max(ch == c0 ? above - 1u : above, lowest);
+      const float past = ch == c0 ? first_thr : thr;
       bool many = false;
-      if (sortable(now) > past) {
+      if (now > past) {
+        uint32_t bits = 0u;  // a bit for each of the 32 logits
 #pragma unroll
-        for (int i = 0; i < VECS; ++i)
-          if (sortable(high_of[i]) > past) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-              const float x = Vec<T>::get(v[i], j);
-              if (sortable(x) > past) {
-                const int at = atomicAdd(&sm.count, 1);
-                if (at < LIST) sm.list[at] = make_key(x, static_cast<uint32_t>((first + i * THREADS) * N - lead + j));
-                many = many || at >= CUT_AT;
-              }
-            }
-          }
-      }
-      if (__syncthreads_or(many)) {
-        const int count = sm.count;
-        if (count > LIST) {
-          above = select_exactly(sm, x0, max(ch * THREADS * VECS * N - lead, 0), min((ch + 1) * THREADS * VECS * N - lead, p.vocab), p.top);
-        } else {
-          keep_largest(sm, count, p.top);
-          above = max(above, static_cast<uint32_t>(sm.kept[p.top - 1] >> 32));
+        for (int i = 0; i < VECS; ++i) bits |= Vec<T>::exceeding(v[i], past) << (i * N);
+        while (bits != 0u) {
+          const int b = __ffs(bits) - 1;
+          bits &= bits - 1u;
+          const int e = (first + b / N * THREADS) * N - lead + b % N;
+          const int at = atomicAdd(&sm.count, 1);
+          if (at < LIST) sm.list[at] = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
+          many = many || at >= THIN_AT;
         }
-        if (tid < p.top) sm.list[tid] = sm.kept[tid];
-        if (tid == 0) sm.count = p.top;
-        __syncthreads();
+      }
+      if (ch == look || ch + 1 == c1) {
+        if (__syncthreads_or(many)) {
+          const int count = sm.count;
+          __syncthreads();
+          uint32_t reach;
+          if (count > LIST) {
+            reach = select_exactly(sm, x0, max(group * THREADS * VECS * N - lead, 0), min((ch + 1) * THREADS * VECS * N - lead, p.vocab), p.top);
+            if (tid < p.top) sm.list[tid] = sm.kept[tid];
+            if (tid == 0) sm.count = p.top;
+            __syncthreads();
+          } else {
+            reach = thin(sm, count, p.top);
+          }
+          thr = fmaxf(thr, from_sortable(reach));
+        }
+        group = ch + 1;
+        look = c0 + 2 * (look - c0) + 1;
       }
     }
 #pragma unroll
