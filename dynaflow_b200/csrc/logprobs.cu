@@ -9,13 +9,12 @@
 // is filled with them, the lower index first.
 //
 // The k largest: a key of 64 bits, the logit made sortable in the upper half and the complement of its index in
-// the lower, is unique, so equal logits come out with the lower index first. A block goes through its part of the
-// row in chunks of 8192 logits. The first chunk gives a threshold: with r = ceil(k / 8), the smallest of the eight
-// warps' r-th largest lane maxima is reached by at least k logits and by few more. Logits above the threshold are put
-// into a list (their order does not matter, the keys decide). The block looks at the list after 1, 2, 4, 8, ... chunks
-// (as many as bring as many logits above the threshold again): a long one is thinned the same way, which raises the
-// threshold. Chunks that bring more than the list can hold (logits that grow along the row, or a great many equal
-// ones) are selected exactly by bisection over the keys instead.
+// the lower, is unique, so equal logits come out with the lower index first. The pass itself only keeps every thread's
+// maximum, the chunk (8192 bf16 or 4096 fp32 logits) it came from, and the largest maximum of its other chunks. With r = ceil(k / 8) the
+// smallest of the eight warps' r-th largest lane maxima is a threshold that at least k logits of the block's part
+// reach and few more do: the threads whose maximum reaches it read that chunk's logits again (all of their chunks if
+// another one reaches it too) and put what reaches it into a list, which is ranked by comparing all pairs. If it does
+// not fit (a great many equal logits), the k largest keys are selected by bisection instead.
 //
 // Bound: HBM, each logit is read once; then the exponentials (16 a clock and SM). The next chunk is fetched while one
 // is worked on. When there are few rows, a row is cut into slices: up to eight are one thread-block cluster, whose
@@ -31,11 +30,10 @@ namespace df {
 namespace logprobs {
 
 constexpr int THREADS = 256;
-constexpr int PER_THREAD = 32;                       // logits of a chunk a thread
-constexpr int CHUNK = THREADS * PER_THREAD;
+constexpr int VECS = 4;                              // 16-byte vectors of a chunk a thread: 8192 bf16 or 4096 fp32 logits a block
+constexpr int CHUNK = THREADS * VECS * 8;
 constexpr int MAX_TOP = 32;
 constexpr int LIST = 512;                            // candidates of a block
-constexpr int THIN_AT = 64;                          // a list that is longer is thinned
 constexpr int MAX_SLICES = 64;
 constexpr int CLUSTER_SLICES = 8;
 constexpr int LONG_SLICE = 16;                       // chunks of a slice above which a row is cut into more than a cluster
@@ -133,10 +131,10 @@ struct Shared {
   u64 list[LIST];
   u64 kept[MAX_TOP];
   uint32_t warp_value[THREADS / 32];
+  float warp_high[THREADS / 32];
   Stats stats[THREADS / 32];
   alignas(8) Stats total;
   int count, sum[2];
-  uint32_t threshold;
 };
 
 // The r-th largest of the lanes' values (equal ones count as often as they occur).
@@ -154,26 +152,6 @@ __device__ __forceinline__ uint32_t rth_of_lanes(uint32_t v, int r, int lane) {
 __device__ __forceinline__ float just_below(float t, uint32_t ulp) {
   const uint32_t b = __float_as_uint(t);
   return __uint_as_float(t > 0.0f ? b - ulp : (t < 0.0f ? b + ulp : 0x80000000u | ulp));
-}
-
-// Leaves what reaches a threshold in the list: with r = ceil(top / 8) the smallest of the warps' r-th largest values,
-// which at least `top` keys reach. Returns its sortable value. `count` (more than THIN_AT, at most LIST) keys; all threads.
-__device__ __forceinline__ uint32_t thin(Shared& sm, int count, int top) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int i0 = lane * (THREADS / 32) + warp, i1 = i0 + THREADS;  // every warp has its share of the keys
-  const u64 k0 = i0 < count ? sm.list[i0] : 0ull, k1 = i1 < count ? sm.list[i1] : 0ull;
-  const uint32_t v0 = static_cast<uint32_t>(k0 >> 32), v1 = static_cast<uint32_t>(k1 >> 32);
-  const uint32_t r = rth_of_lanes(max(v0, v1), (top + THREADS / 32 - 1) / (THREADS / 32), lane);
-  if (lane == 0) sm.warp_value[warp] = r;
-  if (threadIdx.x == 0) sm.count = 0;
-  __syncthreads();
-  uint32_t reach = sm.warp_value[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
-  if (k0 != 0ull && v0 >= reach) sm.list[atomicAdd(&sm.count, 1)] = k0;
-  if (k1 != 0ull && v1 >= reach) sm.list[atomicAdd(&sm.count, 1)] = k1;
-  __syncthreads();
-  return reach;
 }
 
 // Keeps the `top` largest of the list, largest first, in sm.kept (0: fewer than that). All threads; ends with a barrier.
@@ -210,11 +188,16 @@ struct Vec<__nv_bfloat16> {
     uint32_t& w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
     w = (j & 1) != 0 ? (w & 0xffffu) | bits << 16 : (w & 0xffff0000u) | bits;
   }
-  // largest of the vector's logits (NaN does not count)
-  static __device__ __forceinline__ float highest(const uint4& v) {
-    const __nv_bfloat162 a = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.x), reinterpret_cast<const __nv_bfloat162&>(v.y));
-    const __nv_bfloat162 b = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.z), reinterpret_cast<const __nv_bfloat162&>(v.w));
-    const __nv_bfloat162 m = __hmax2(a, b);
+  // largest of the vectors' logits (NaN does not count)
+  template <int COUNT>
+  static __device__ __forceinline__ float highest(const uint4 (&v)[COUNT]) {
+    __nv_bfloat162 m = __float2bfloat162_rn(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const __nv_bfloat162 a = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v[i].x), reinterpret_cast<const __nv_bfloat162&>(v[i].y));
+      const __nv_bfloat162 b = __hmax2(reinterpret_cast<const __nv_bfloat162&>(v[i].z), reinterpret_cast<const __nv_bfloat162&>(v[i].w));
+      m = __hmax2(m, __hmax2(a, b));
+    }
     return fmaxf(__low2float(m), __high2float(m));
   }
   // pair i of the vector, no lower than LOWEST (NaN stays)
@@ -238,7 +221,13 @@ struct Vec<float> {
     return (get(v, 0) > thr ? 1u : 0u) | (get(v, 1) > thr ? 2u : 0u) | (get(v, 2) > thr ? 4u : 0u) | (get(v, 3) > thr ? 8u : 0u);
   }
   static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) { (j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w) = bits; }
-  static __device__ __forceinline__ float highest(const uint4& v) { return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3))); }
+  template <int COUNT>
+  static __device__ __forceinline__ float highest(const uint4 (&v)[COUNT]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) m = fmaxf(m, fmaxf(fmaxf(get(v[i], 0), get(v[i], 1)), fmaxf(get(v[i], 2), get(v[i], 3))));
+    return m;
+  }
   static __device__ __forceinline__ float lift(float x) {  // max that keeps NaN
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(LOWEST));
@@ -273,38 +262,39 @@ __device__ __forceinline__ void write_record(const Params& p, int part, int row,
     reinterpret_cast<u64*>(base + static_cast<size_t>(p.rows) * sizeof(Stats))[static_cast<size_t>(row) * p.top + threadIdx.x] = kept[threadIdx.x];
 }
 
-// A chunk of this thread's logits, 16-byte vectors; what lies outside the row is -inf.
+// A chunk of this thread's logits, 16-byte vectors from element `e` (THREADS vectors apart); outside the row: -inf.
 template <typename T>
-__device__ __forceinline__ void load_chunk(uint4 (&v)[PER_THREAD / Vec<T>::N], const T* x0, int first, int lead, int vocab) {
+__device__ __forceinline__ void load_chunk(uint4 (&v)[VECS], const T* x0, int e, int vocab, bool inside) {
   constexpr int N = Vec<T>::N;
+  if (inside) {  // the whole block's chunk
+    const uint4* src = reinterpret_cast<const uint4*>(x0 + e);
 #pragma unroll
-  for (int i = 0; i < PER_THREAD / N; ++i) {
-    const int e = (first + i * THREADS) * N - lead;  // first element of the vector
-    if (e >= 0 && e + N <= vocab) {
-      v[i] = __ldg(reinterpret_cast<const uint4*>(x0 + e));
-    } else {
-      v[i] = make_uint4(Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN);
+    for (int i = 0; i < VECS; ++i) v[i] = __ldg(src + i * THREADS);
+  } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (e + j >= 0 && e + j < vocab) Vec<T>::put(v[i], j, Vec<T>::raw(x0 + e + j));
+    for (int i = 0; i < VECS; ++i, e += THREADS * N) {
+      if (e >= 0 && e + N <= vocab) {
+        v[i] = __ldg(reinterpret_cast<const uint4*>(x0 + e));
+      } else {
+        v[i] = make_uint4(Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (e + j >= 0 && e + j < vocab) Vec<T>::put(v[i], j, Vec<T>::raw(x0 + e + j));
+      }
     }
   }
 }
 
-// A chunk (elements [e0, e1) of the row) with more candidates than the list holds: the `top` largest keys of it and of
-// what the list held before it, exactly, by bisection. They replace the list; returns the smallest one's value. (Reads
-// the chunk again: rows of equal or of rising logits come here, others do not.) All threads.
+// More candidates among elements [e0, e1) of the row than the list holds: the `top` largest keys, exactly, by bisection;
+// they replace the list. (Goes through the elements 64 times: rows of equal logits come here, others do not.) All threads.
 template <typename T>
-__device__ __noinline__ uint32_t select_exactly(Shared& sm, const T* x0, int e0, int e1, int top) {
+__device__ __noinline__ void select_exactly(Shared& sm, const T* x0, int e0, int e1, int top) {
   const int tid = threadIdx.x;
-  // the list is full; its entries of this chunk are in the chunk too: only those with an index before it count
-  auto older = [&](u64 key) { return 0xffffffffu - static_cast<uint32_t>(key) < static_cast<uint32_t>(e0); };
   u64 found = 0ull;
   for (int bit = 63; bit >= 0; --bit) {
     const u64 mid = found | (1ull << bit);
     int n = 0;
     for (int e = e0 + tid; e < e1; e += THREADS) n += make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e)) >= mid ? 1 : 0;
-    for (int i = tid; i < LIST; i += THREADS) n += sm.list[i] >= mid && older(sm.list[i]) ? 1 : 0;
     if (tid == 0) sm.sum[bit & 1] = 0;
     __syncthreads();
     n = __reduce_add_sync(0xffffffffu, n);
@@ -314,14 +304,11 @@ __device__ __noinline__ uint32_t select_exactly(Shared& sm, const T* x0, int e0,
   }
   if (tid == 0) sm.count = 0;
   __syncthreads();
-  for (int i = tid; i < LIST; i += THREADS)
-    if (sm.list[i] >= found && older(sm.list[i])) sm.kept[atomicAdd(&sm.count, 1)] = sm.list[i];
   for (int e = e0 + tid; e < e1; e += THREADS) {
     const u64 key = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
-    if (key >= found) sm.kept[atomicAdd(&sm.count, 1)] = key;
+    if (key >= found) sm.list[atomicAdd(&sm.count, 1)] = key;
   }
   __syncthreads();
-  return static_cast<uint32_t>(found >> 32);
 }
 
 // The list has fewer than `top` keys because the other logits of elements [e0, e1) are forbidden (at or below LOWEST):
@@ -374,8 +361,8 @@ __device__ __forceinline__ u64 read_remote(const u64* p, unsigned rank) {
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprobs_kernel(const Params p) {
-  constexpr int N = Vec<T>::N, VECS = PER_THREAD / N;
+__global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params p) {
+  constexpr int N = Vec<T>::N;
   __shared__ Shared sm;
   grid_dependency_wait();
   grid_launch_dependents();
@@ -393,24 +380,16 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
     if (id >= 0 && id < p.vocab) given = Vec<T>::one(x0 + id);
   }
   if (TOP && tid == 0) sm.count = 0;
-  float high = -INFINITY;                 // largest logit of this thread
+  float high = -INFINITY, other = -INFINITY;  // largest logit of this thread; largest of the chunks that it is not from
+  int high_chunk = c0;
   u64 s2 = pack2(0.f, 0.f), u2 = s2;
-  float thr = LOWEST;                     // a candidate exceeds it
-  int look = c0, group = c0;              // the list is looked at after chunk `look`; first chunk since the last look
   const u64 scale = pack2(LOG2E, LOG2E);
-  uint4 v[VECS];
-  if (c0 < c1) load_chunk<T>(v, x0, c0 * THREADS * VECS + tid, lead, p.vocab);
-  for (int ch = c0; ch < c1; ++ch) {
-    uint4 ahead[VECS];
-    const int first = ch * THREADS * VECS + tid;
-    if (ch + 1 < c1) load_chunk<T>(ahead, x0, first + THREADS * VECS, lead, p.vocab);
-    float high_of[VECS], now = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      high_of[i] = Vec<T>::highest(v[i]);
-      now = fmaxf(now, high_of[i]);
-    }
-    // ---- sums
+  constexpr int STEP = THREADS * VECS * N;  // elements of a chunk
+  auto element = [&](int ch) { return ch * STEP + tid * N - lead; };
+  auto load = [&](uint4 (&v)[VECS], int ch) { load_chunk<T>(v, x0, element(ch), p.vocab, ch * STEP >= lead && (ch + 1) * STEP - lead <= p.vocab); };
+  auto work = [&](const uint4 (&v)[VECS], int ch) {
+    const float now = Vec<T>::highest(v);
+    if (TOP) other = fmaxf(other, fminf(now, high));
     if (now > high) {
       if (high > LOWEST) {
         const float d = (high - now) * LOG2E, f = ex2f(d);
@@ -419,9 +398,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
         u2 = pack2(f * fmaf(d, s.x, u.x), f * fmaf(d, s.y, u.y));
       }
       high = now;
+      high_chunk = ch;
     }
-    const float ref = high > LOWEST ? high : 0.0f;  // without a reference 2^(LOWEST) is 0, too
-    const u64 minus = pack2(-ref, -ref);
+    const float ref = high > LOWEST ? -high : 0.0f;  // without a reference 2^(LOWEST) is 0, too
+    const u64 minus = pack2(ref, ref);
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
@@ -432,59 +412,20 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
         s2 = add2(s2, e);
         u2 = fma2(e, y, u2);
       }
-    // ---- candidates
-    if (TOP) {
-      float first_thr = LOWEST;
-      if (ch == c0) {
-        const uint32_t r = rth_of_lanes(sortable(now), (p.top + THREADS / 32 - 1) / (THREADS / 32), lane);
-        if (lane == 0) sm.warp_value[warp] = r;
-        __syncthreads();
-        uint32_t reach = sm.warp_value[0];
-#pragma unroll
-        for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
-        // the first chunk takes what reaches this; later logits have higher indices: those equal to it lose
-        thr = fmaxf(from_sortable(reach), LOWEST);
-        if (thr > LOWEST) first_thr = just_below(thr, Vec<T>::ULP);
-      }
-      const float past = ch == c0 ? first_thr : thr;
-      bool many = false;
-      if (now > past) {
-        uint32_t bits = 0u;  // a bit for each of the 32 logits
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) bits |= Vec<T>::exceeding(v[i], past) << (i * N);
-        while (bits != 0u) {
-          const int b = __ffs(bits) - 1;
-          bits &= bits - 1u;
-          const int e = (first + b / N * THREADS) * N - lead + b % N;
-          const int at = atomicAdd(&sm.count, 1);
-          if (at < LIST) sm.list[at] = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
-          many = many || at >= THIN_AT;
-        }
-      }
-      if (ch == look || ch + 1 == c1) {
-        if (__syncthreads_or(many)) {
-          const int count = sm.count;
-          __syncthreads();
-          uint32_t reach;
-          if (count > LIST) {
-            reach = select_exactly(sm, x0, max(group * THREADS * VECS * N - lead, 0), min((ch + 1) * THREADS * VECS * N - lead, p.vocab), p.top);
-            if (tid < p.top) sm.list[tid] = sm.kept[tid];
-            if (tid == 0) sm.count = p.top;
-            __syncthreads();
-          } else {
-            reach = thin(sm, count, p.top);
-          }
-          thr = fmaxf(thr, from_sortable(reach));
-        }
-        group = ch + 1;
-        look = c0 + 2 * (look - c0) + 1;
-      }
+  };
+  uint4 va[VECS], vb[VECS];  // one chunk is on its way while the other is worked on
+  load(va, c0);
+  for (int ch = c0; ch < c1; ch += 2) {
+    if (ch + 1 < c1) load(vb, ch + 1);
+    work(va, ch);
+    if (ch + 1 < c1) {
+      if (ch + 2 < c1) load(va, ch + 2);
+      work(vb, ch + 1);
     }
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) v[i] = ahead[i];
   }
   // ---- the block's sums
   const float2 s = unpack2(s2), u = unpack2(u2);
+  const float mine = high;
   Stats st{-INFINITY, 0.0f, 0.0f, given};
   if (high > LOWEST) {
     st.m = high;
@@ -498,15 +439,39 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
     join(st, shuffle(st, o));
     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
   }
+  const uint32_t rth = TOP ? rth_of_lanes(sortable(mine), (p.top + THREADS / 32 - 1) / (THREADS / 32), lane) : 0u;
   if (lane == 0) {
     sm.stats[warp] = st;
-    sm.warp_value[warp] = __float_as_uint(high);
+    sm.warp_high[warp] = high;
+    sm.warp_value[warp] = rth;
   }
   __syncthreads();
-  const int e0 = max(c0 * THREADS * VECS * N - lead, 0), e1 = min(c1 * THREADS * VECS * N - lead, p.vocab);
+  const int e0 = max(c0 * STEP - lead, 0), e1 = min(c1 * STEP - lead, p.vocab);
+  if (TOP) {
+    uint32_t reach = sm.warp_value[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
+    const float least = from_sortable(reach), past = least > LOWEST ? just_below(least, Vec<T>::ULP) : LOWEST;  // a candidate exceeds it
+    if (mine > past) {
+      const bool all = other > past;
+      for (int ch = all ? c0 : high_chunk; ch < (all ? c1 : high_chunk + 1); ++ch) {
+        load(va, ch);
+        uint32_t bits = 0u;  // a bit for each of the chunk's logits of this thread
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) bits |= Vec<T>::exceeding(va[i], past) << (i * N);
+        while (bits != 0u) {
+          const int b = __ffs(bits) - 1, e = element(ch) + b / N * (THREADS * N) + b % N;
+          const int at = atomicAdd(&sm.count, 1);
+          if (at < LIST) sm.list[at] = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
+          bits = at < LIST ? bits & (bits - 1u) : 0u;
+        }
+        if (sm.count > LIST) break;
+      }
+    }
+  }
   if (warp == 0) {
     st = sm.stats[lane & 7];
-    high = __uint_as_float(sm.warp_value[lane & 7]);
+    high = sm.warp_high[lane & 7];
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) {
       join(st, shuffle(st, o));
@@ -534,6 +499,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) token_logprob
     if (lane == 0) sm.total = st;
   }
   if (TOP) {
+    __syncthreads();
+    if (sm.count > LIST) select_exactly(sm, x0, e0, e1, p.top);
     if (sm.count < p.top) fill_forbidden(sm, x0, e0, e1, p.top);
     keep_largest(sm, min(sm.count, LIST), p.top);
   } else {
