@@ -9,12 +9,12 @@
 // is filled with them, the lower index first.
 //
 // The k largest: a key of 64 bits, the logit made sortable in the upper half and the complement of its index in
-// the lower, is unique, so equal logits come out with the lower index first. The pass itself only keeps every thread's
-// maximum, the chunk (8192 bf16 or 4096 fp32 logits) it came from, and the largest maximum of its other chunks. With r = ceil(k / 8) the
-// smallest of the eight warps' r-th largest lane maxima is a threshold that at least k logits of the block's part
-// reach and few more do: the threads whose maximum reaches it read that chunk's logits again (all of their chunks if
-// another one reaches it too) and put what reaches it into a list, which is ranked by comparing all pairs. If it does
-// not fit (a great many equal logits), the k largest keys are selected by bisection instead.
+// the lower, is unique, so equal logits come out with the lower index first. The pass itself only leaves every
+// thread's maximum of each of at most 16 stretches of its part (as bf16, rounded up) in shared memory. With
+// r = ceil(k / 8) the smallest of the eight warps' r-th largest lane maxima is a threshold that at least k logits of
+// the block's part reach and few more do: the threads with a stretch that reaches it read that stretch again and put
+// what reaches it into a list, which is ranked by comparing all pairs. If it does not fit (a great many equal logits),
+// the k largest keys are selected by bisection instead.
 //
 // Bound: HBM, each logit is read once; then the exponentials (16 a clock and SM). The next chunk is fetched while one
 // is worked on. When there are few rows, a row is cut into slices: up to eight are one thread-block cluster, whose
@@ -127,14 +127,17 @@ __device__ __forceinline__ Stats shuffle(const Stats& v, int o) {
   return r;
 }
 
+constexpr int STRETCHES = 16;
 struct Shared {
+  __nv_bfloat16 stretch[STRETCHES][THREADS];
   u64 list[LIST];
   u64 kept[MAX_TOP];
   uint32_t warp_value[THREADS / 32];
   float warp_high[THREADS / 32];
   Stats stats[THREADS / 32];
   alignas(8) Stats total;
-  int count, sum[2];
+  uint32_t items[LIST];  // (stretch << 8 | thread) with a candidate
+  int count, item_count, sum[2];
 };
 
 // The r-th largest of the lanes' values (equal ones count as often as they occur).
@@ -154,15 +157,20 @@ __device__ __forceinline__ float just_below(float t, uint32_t ulp) {
   return __uint_as_float(t > 0.0f ? b - ulp : (t < 0.0f ? b + ulp : 0x80000000u | ulp));
 }
 
-// Keeps the `top` largest of the list, largest first, in sm.kept (0: fewer than that). All threads; ends with a barrier.
+// Keeps the `top` largest of the list, largest first, in sm.kept (0: fewer than that): a key's place is the number of
+// larger ones, counted by four threads. All threads; ends with a barrier.
 __device__ __forceinline__ void keep_largest(Shared& sm, int count, int top) {
   if (threadIdx.x < MAX_TOP) sm.kept[threadIdx.x] = 0ull;
   __syncthreads();
-  for (int i = threadIdx.x; i < count; i += THREADS) {
+  const unsigned quad = 0xfu << (threadIdx.x & 28);
+  for (int i = threadIdx.x >> 2; i < count; i += THREADS / 4) {
     const u64 key = sm.list[i];
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += sm.list[j] > key ? 1 : 0;
-    if (rank < top) sm.kept[rank] = key;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < count; j += 4) rank += sm.list[j] > key ? 1 : 0;
+    rank += __shfl_xor_sync(quad, rank, 1);
+    rank += __shfl_xor_sync(quad, rank, 2);
+    if (rank < top && (threadIdx.x & 3) == 0) sm.kept[rank] = key;
   }
   __syncthreads();
 }
@@ -175,7 +183,10 @@ struct Vec<__nv_bfloat16> {
   static constexpr uint32_t FORBIDDEN = 0xff80ff80u;  // -inf, twice
   static constexpr uint32_t ULP = 0x10000u;           // of the fp32 bits of a logit
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ uint32_t raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint16_t*>(p); }
+  static __device__ __forceinline__ float get(const uint4& v, int j) {
+    const uint32_t w = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
+    return __uint_as_float((j & 1) != 0 ? w & 0xffff0000u : w << 16);
+  }
   // bit j of the result: whether logit j of the vector exceeds thr
   static __device__ __forceinline__ uint32_t exceeding(const uint4& v, float thr) {
     const __nv_bfloat162 t = __float2bfloat162_rn(thr);
@@ -183,10 +194,6 @@ struct Vec<__nv_bfloat16> {
     const uint32_t c = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.z), t), d = __hgt2_mask(reinterpret_cast<const __nv_bfloat162&>(v.w), t);
     const uint32_t m = (a & 0x00010001u) | (b & 0x00040004u) | (c & 0x00100010u) | (d & 0x00400040u);  // 2 i and 16 + 2 i
     return (m | m >> 15) & 0xffu;
-  }
-  static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) {
-    uint32_t& w = (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w;
-    w = (j & 1) != 0 ? (w & 0xffffu) | bits << 16 : (w & 0xffff0000u) | bits;
   }
   // largest of the vectors' logits (NaN does not count)
   template <int COUNT>
@@ -215,12 +222,10 @@ struct Vec<float> {
   static constexpr uint32_t FORBIDDEN = 0xff800000u;
   static constexpr uint32_t ULP = 1u;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
-  static __device__ __forceinline__ uint32_t raw(const float* p) { return __float_as_uint(*p); }
-  static __device__ __forceinline__ float get(const uint4& v, int j) { return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w); }
+  static __device__ __forceinline__ float get(const uint4& v, int j) { return __uint_as_float(j < 2 ? (j == 0 ? v.x : v.y) : (j == 2 ? v.z : v.w)); }
   static __device__ __forceinline__ uint32_t exceeding(const uint4& v, float thr) {
     return (get(v, 0) > thr ? 1u : 0u) | (get(v, 1) > thr ? 2u : 0u) | (get(v, 2) > thr ? 4u : 0u) | (get(v, 3) > thr ? 8u : 0u);
   }
-  static __device__ __forceinline__ void put(uint4& v, int j, uint32_t bits) { (j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w) = bits; }
   template <int COUNT>
   static __device__ __forceinline__ float highest(const uint4 (&v)[COUNT]) {
     float m = -INFINITY;
@@ -237,7 +242,7 @@ struct Vec<float> {
 };
 
 // From base 2 with the fp32 constant LOG2E, whose powers are those of e to 2^-26 of the exponent.
-__device__ __forceinline__ float to_nats(double bits) { return static_cast<float>(bits / static_cast<double>(LOG2E)); }
+__device__ __forceinline__ float to_nats(double bits) { return static_cast<float>(bits * (1.0 / static_cast<double>(LOG2E))); }
 __device__ __forceinline__ float logprob_of(float x, const Stats& s, float log_s) {
   return to_nats((static_cast<double>(x) - static_cast<double>(s.m)) * static_cast<double>(LOG2E) - static_cast<double>(log_s));
 }
@@ -262,25 +267,17 @@ __device__ __forceinline__ void write_record(const Params& p, int part, int row,
     reinterpret_cast<u64*>(base + static_cast<size_t>(p.rows) * sizeof(Stats))[static_cast<size_t>(row) * p.top + threadIdx.x] = kept[threadIdx.x];
 }
 
-// A chunk of this thread's logits, 16-byte vectors from element `e` (THREADS vectors apart); outside the row: -inf.
+// A chunk of this thread's logits: vectors `at`, at + THREADS, ... of `vectors`; behind the last one -inf.
 template <typename T>
-__device__ __forceinline__ void load_chunk(uint4 (&v)[VECS], const T* x0, int e, int vocab, bool inside) {
-  constexpr int N = Vec<T>::N;
-  if (inside) {  // the whole block's chunk
-    const uint4* src = reinterpret_cast<const uint4*>(x0 + e);
+__device__ __forceinline__ void load_chunk(uint4 (&v)[VECS], const uint4* src, int at, int vectors, bool full) {
+  if (full) {  // the whole block's chunk
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) v[i] = __ldg(src + i * THREADS);
+    for (int i = 0; i < VECS; ++i) v[i] = __ldg(src + at + i * THREADS);
   } else {
 #pragma unroll
-    for (int i = 0; i < VECS; ++i, e += THREADS * N) {
-      if (e >= 0 && e + N <= vocab) {
-        v[i] = __ldg(reinterpret_cast<const uint4*>(x0 + e));
-      } else {
-        v[i] = make_uint4(Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (e + j >= 0 && e + j < vocab) Vec<T>::put(v[i], j, Vec<T>::raw(x0 + e + j));
-      }
+    for (int i = 0; i < VECS; ++i) {
+      v[i] = make_uint4(Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN, Vec<T>::FORBIDDEN);
+      if (at + i * THREADS < vectors) v[i] = __ldg(src + at + i * THREADS);
     }
   }
 }
@@ -294,6 +291,7 @@ __device__ __noinline__ void select_exactly(Shared& sm, const T* x0, int e0, int
   for (int bit = 63; bit >= 0; --bit) {
     const u64 mid = found | (1ull << bit);
     int n = 0;
+#pragma unroll 1
     for (int e = e0 + tid; e < e1; e += THREADS) n += make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e)) >= mid ? 1 : 0;
     if (tid == 0) sm.sum[bit & 1] = 0;
     __syncthreads();
@@ -369,27 +367,41 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
   const int row = blockIdx.x / p.slices, slice = blockIdx.x - row * p.slices;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x0 = static_cast<const T*>(p.logits) + row * p.ld;
-  // vectors lie on 16-byte boundaries; the row begins `lead` elements into its first one
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x0) & 15u) / sizeof(T));
-  const int vectors = (p.vocab + lead + N - 1) / N;
+  // whole vectors on 16-byte boundaries from element `head`; the few logits before and behind them are a thread's each
+  const int head = min(static_cast<int>((16u - (reinterpret_cast<uintptr_t>(x0) & 15u)) % 16u / sizeof(T)), p.vocab);
+  const int vectors = (p.vocab - head) / N;
+  const uint4* src = reinterpret_cast<const uint4*>(x0 + head);
   const int chunks = (vectors + THREADS * VECS - 1) / (THREADS * VECS);
-  const int c0 = static_cast<int>(static_cast<long long>(chunks) * slice / p.slices), c1 = static_cast<int>(static_cast<long long>(chunks) * (slice + 1) / p.slices);
+  const int c0 = chunks * slice / p.slices, c1 = chunks * (slice + 1) / p.slices;
+  float extra = -INFINITY;
+  int extra_at = 0;
+  if (tid < 16 && slice == (tid < 8 ? 0 : p.slices - 1)) {
+    extra_at = tid < 8 ? tid : head + vectors * N + tid - 8;
+    if (extra_at < (tid < 8 ? head : p.vocab)) extra = Vec<T>::one(x0 + extra_at);
+  }
   float given = -INFINITY;
   if (slice == 0 && tid == 0) {
     const long long id = (p.id_bytes == 8 ? static_cast<const long long*>(p.ids)[row] : static_cast<const int*>(p.ids)[row]) - p.vocab_start;
     if (id >= 0 && id < p.vocab) given = Vec<T>::one(x0 + id);
   }
-  if (TOP && tid == 0) sm.count = 0;
-  float high = -INFINITY, other = -INFINITY;  // largest logit of this thread; largest of the chunks that it is not from
-  int high_chunk = c0;
+  if (TOP && tid == 0) sm.count = sm.item_count = 0;
+  float high = -INFINITY;  // largest logit of this thread
   u64 s2 = pack2(0.f, 0.f), u2 = s2;
   const u64 scale = pack2(LOG2E, LOG2E);
-  constexpr int STEP = THREADS * VECS * N;  // elements of a chunk
-  auto element = [&](int ch) { return ch * STEP + tid * N - lead; };
-  auto load = [&](uint4 (&v)[VECS], int ch) { load_chunk<T>(v, x0, element(ch), p.vocab, ch * STEP >= lead && (ch + 1) * STEP - lead <= p.vocab); };
+  auto load = [&](uint4 (&v)[VECS], int ch) { load_chunk<T>(v, src, ch * (THREADS * VECS) + tid, vectors, (ch + 1) * (THREADS * VECS) <= vectors); };
+  const int per_stretch = max((c1 - c0 + STRETCHES - 1) / STRETCHES, 1);  // chunks
+  float stretch_high = -INFINITY;
+  int in_stretch = 0;
   auto work = [&](const uint4 (&v)[VECS], int ch) {
     const float now = Vec<T>::highest(v);
-    if (TOP) other = fmaxf(other, fminf(now, high));
+    if (TOP) {
+      stretch_high = fmaxf(stretch_high, now);
+      if (++in_stretch == per_stretch || ch + 1 == c1) {
+        sm.stretch[(ch - c0) / per_stretch][tid] = __float2bfloat16_ru(stretch_high);
+        stretch_high = -INFINITY;
+        in_stretch = 0;
+      }
+    }
     if (now > high) {
       if (high > LOWEST) {
         const float d = (high - now) * LOG2E, f = ex2f(d);
@@ -398,7 +410,6 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
         u2 = pack2(f * fmaf(d, s.x, u.x), f * fmaf(d, s.y, u.y));
       }
       high = now;
-      high_chunk = ch;
     }
     const float ref = high > LOWEST ? -high : 0.0f;  // without a reference 2^(LOWEST) is 0, too
     const u64 minus = pack2(ref, ref);
@@ -414,7 +425,8 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
       }
   };
   uint4 va[VECS], vb[VECS];  // one chunk is on its way while the other is worked on
-  load(va, c0);
+  if (c0 < c1) load(va, c0);
+#pragma unroll 1
   for (int ch = c0; ch < c1; ch += 2) {
     if (ch + 1 < c1) load(vb, ch + 1);
     work(va, ch);
@@ -425,7 +437,6 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
   }
   // ---- the block's sums
   const float2 s = unpack2(s2), u = unpack2(u2);
-  const float mine = high;
   Stats st{-INFINITY, 0.0f, 0.0f, given};
   if (high > LOWEST) {
     st.m = high;
@@ -434,6 +445,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
   } else if (s.x + s.y != s.x + s.y) {
     st.s = NAN;  // a NaN among forbidden tokens
   }
+  if (extra > LOWEST) join(st, Stats{extra, 1.0f, 0.0f, -INFINITY});
+  if (extra != extra) st.s = NAN;
+  high = fmaxf(high, extra);
+  const float mine = high;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     join(st, shuffle(st, o));
@@ -446,26 +461,43 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
     sm.warp_value[warp] = rth;
   }
   __syncthreads();
-  const int e0 = max(c0 * STEP - lead, 0), e1 = min(c1 * STEP - lead, p.vocab);
+  // this block's logits; the first slice has those before the first vector, the last one those behind the last
+  const int e0 = slice == 0 ? 0 : head + c0 * (THREADS * VECS * N), e1 = slice == p.slices - 1 ? p.vocab : head + c1 * (THREADS * VECS * N);
   if (TOP) {
     uint32_t reach = sm.warp_value[0];
 #pragma unroll
     for (int i = 1; i < THREADS / 32; ++i) reach = min(reach, sm.warp_value[i]);
     const float least = from_sortable(reach), past = least > LOWEST ? just_below(least, Vec<T>::ULP) : LOWEST;  // a candidate exceeds it
+    auto append = [&](float x, int e) {
+      const int at = atomicAdd(&sm.count, 1);
+      if (at < LIST) sm.list[at] = make_key(x, static_cast<uint32_t>(e));
+    };
     if (mine > past) {
-      const bool all = other > past;
-      for (int ch = all ? c0 : high_chunk; ch < (all ? c1 : high_chunk + 1); ++ch) {
-        load(va, ch);
-        uint32_t bits = 0u;  // a bit for each of the chunk's logits of this thread
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) bits |= Vec<T>::exceeding(va[i], past) << (i * N);
-        while (bits != 0u) {
-          const int b = __ffs(bits) - 1, e = element(ch) + b / N * (THREADS * N) + b % N;
-          const int at = atomicAdd(&sm.count, 1);
-          if (at < LIST) sm.list[at] = make_key(Vec<T>::one(x0 + e), static_cast<uint32_t>(e));
-          bits = at < LIST ? bits & (bits - 1u) : 0u;
+      if (extra > past) append(extra, extra_at);
+      const int stretches = (c1 - c0 + per_stretch - 1) / per_stretch;
+#pragma unroll 4
+      for (int i = 0; i < stretches; ++i)
+        if (__bfloat162float(sm.stretch[i][tid]) > past) {  // (or only seems so when rounded up)
+          const int at = atomicAdd(&sm.item_count, 1);
+          if (at < LIST) sm.items[at] = static_cast<uint32_t>(i << 8 | tid);
         }
-        if (sm.count > LIST) break;
+    }
+    __syncthreads();
+    const int items = sm.item_count;
+    if (items > LIST) {
+      if (tid == 0) sm.count = LIST + 1;
+    } else {
+      for (int w = tid; w < items * VECS * per_stretch; w += THREADS) {
+        const int item = w / (VECS * per_stretch), rest = w - item * (VECS * per_stretch);
+        const int i = static_cast<int>(sm.items[item] >> 8), thread = static_cast<int>(sm.items[item] & 255u);
+        const int ch = c0 + i * per_stretch + rest / VECS, at = ch * (THREADS * VECS) + rest % VECS * THREADS + thread;
+        if (ch >= c1 || at >= vectors) continue;
+        const uint4 v = __ldg(src + at);
+#pragma unroll 1
+        for (uint32_t bits = Vec<T>::exceeding(v, past); bits != 0u; bits &= bits - 1u) {
+          const int j = __ffs(bits) - 1;
+          append(Vec<T>::get(v, j), head + at * N + j);
+        }
       }
     }
   }
@@ -482,12 +514,13 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Params
       const bool nan = st.s != st.s;
       float sum = 0.0f, moment = 0.0f;
       if (high > -INFINITY)
+#pragma unroll 1
         for (int e = e0 + lane; e < e1; e += 32) {
           const float y = (Vec<T>::one(x0 + e) - high) * LOG2E, w = ex2f(y);
           sum += w;
           if (w > 0.0f) moment = fmaf(w, y, moment);
         }
-#pragma unroll
+#pragma unroll 1
       for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
         moment += __shfl_xor_sync(0xffffffffu, moment, o);
