@@ -938,8 +938,15 @@ int launch_attention(const AttnParams& p, int grid, cudaStream_t s) {
   using Shared = AttnShared<NT, WARPS, STAGES>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of an SM");
   auto kernel = attention_paged4_kernel<NT, WARPS, STAGES>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
-  if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(WARPS * 32, 1, 1);

@@ -87,6 +87,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
   grid_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int worker = blockIdx.x * PLAN_THREADS + tid, workers = gridDim.x * PLAN_THREADS;
+  const int count = min(max(p.free_count[0], 0), p.num_pages);
+  auto everyone = [&]() {  // one cluster, or one CTA
+    if (gridDim.x > 1) cluster_sync();
+    else __syncthreads();
+  };
 
   int carry[3] = {0, 0, 0};
   for (int b0 = 0; b0 < p.requests; b0 += PLAN_THREADS) {
@@ -133,7 +138,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
   }
   if (tid < 3) sums[tid * (p.requests + 1) + p.requests] = carry[tid];
   __syncthreads();
-  const int count = min(max(p.free_count[0], 0), p.num_pages);
   const int taken = carry[1], returned = carry[2];
   const int top = count + returned;
   const bool enough = taken <= top;
@@ -147,7 +151,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
     if (to < p.num_pages) p.free_pages[to] = *entry;
     *entry = -1;
   }
-  cluster_sync();  // the list is complete
+  if (returned > 0) everyone();  // the list is complete
 
   // pages taken: into the tables
   if (enough)
@@ -157,30 +161,57 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
       const int from = top - 1 - i;
       p.table[static_cast<size_t>(b) * p.max_pages + r.held + (i - more_at[b])] = from < p.num_pages ? p.free_pages[from] : -1;
     }
-  // rows: the request of a row from the prefix sums; a page that this launch hands out is read from the list, not from
-  // the table (another thread may be writing that entry)
-  for (int row = worker; row < p.rows; row += workers) {
-    const int b = p.rows_per_request > 0 ? min(row / p.rows_per_request, p.requests - 1) : find_last(row_at, p.requests, row);
-    const Request r = load_request(p, b);
-    const int i = row - row_at[b];
-    int slot = -1, position = 0;
-    if (i < (p.rows_per_request > 0 ? min(r.fresh, p.rows_per_request) : r.fresh)) {
-      position = r.len - r.fresh + i;
-      const int column = position / p.page_size;
-      int page = -1;
-      if (column < min(r.held, r.need)) {
-        page = p.table[static_cast<size_t>(b) * p.max_pages + column];
-      } else if (enough && column < r.need) {
-        const int from = top - 1 - (more_at[b] + column - r.held);
-        page = from < p.num_pages ? p.free_pages[from] : -1;
+  // Rows, four a thread: the request of the first one from the prefix sums, the others from there. A page that this launch
+  // hands out is read from the list, not from the table (another thread may be writing that entry).
+  const bool whole = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15u) == 0;
+  for (int row0 = 4 * worker; row0 < p.rows; row0 += 4 * workers) {
+    int b = p.rows_per_request > 0 ? min(row0 / p.rows_per_request, p.requests - 1) : find_last(row_at, p.requests, row0);
+    Request r = load_request(p, b);
+    int4 slot4, position4;
+    int* slots = &slot4.x;
+    int* positions = &position4.x;
+    int column = -1, page = -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = row0 + k;
+      while (b + 1 < p.requests && row >= row_at[b + 1]) {
+        r = load_request(p, ++b);
+        column = -1;
       }
-      if (page >= 0 && page < p.num_pages) slot = page * p.page_size + position % p.page_size;
+      const int i = row - row_at[b];
+      int slot = -1, position = 0;
+      if (i < (p.rows_per_request > 0 ? min(r.fresh, p.rows_per_request) : r.fresh)) {
+        position = r.len - r.fresh + i;
+        const int c = position / p.page_size;
+        if (c != column) {
+          column = c;
+          page = -1;
+          if (c < min(r.held, r.need)) {
+            page = p.table[static_cast<size_t>(b) * p.max_pages + c];
+          } else if (enough && c < r.need) {
+            const int from = top - 1 - (more_at[b] + c - r.held);
+            page = from < p.num_pages ? p.free_pages[from] : -1;
+          }
+        }
+        if (page >= 0 && page < p.num_pages) slot = page * p.page_size + (position - c * p.page_size);
+      }
+      slots[k] = slot;
+      positions[k] = position;
     }
-    p.slots[row] = slot;
-    p.positions[row] = position;
+    if (whole && row0 + 4 <= p.rows) {
+      *reinterpret_cast<int4*>(p.slots + row0) = slot4;
+      *reinterpret_cast<int4*>(p.positions + row0) = position4;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (row0 + k < p.rows) {
+          p.slots[row0 + k] = slots[k];
+          p.positions[row0 + k] = positions[k];
+        }
+    }
   }
   for (int b = worker; b <= p.requests; b += workers) p.row_starts[b] = row_at[b];
-  cluster_sync();  // every CTA is done with the old state
+  everyone();  // every thread is done with the old state
   for (int b = worker; b < p.requests; b += workers) {
     const Request r = load_request(p, b);
     if (r.need <= r.held || enough) p.held[b] = r.need;
@@ -201,11 +232,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
 //
 // Rounding points: the rotated value is rounded to bf16 (it is the bf16 key that is quantised); scale =
 // bf16(max / 15 - min / 15); code = (x - min) / scale rounded to nearest even; every operation is the IEEE
-// one (no contraction, no approximate division), so the codes are the same on any machine.
+// one (no contraction, no approximate division), so the codes are the same on any machine. The quotient is
+// Markstein's: with r = 1 / scale correctly rounded and t = d r, t + (d - t scale) r in two fused operations is the
+// correctly rounded d / scale (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990);
+// scales so small or large that a step could leave the normal numbers take the division itself.
 //
 // Bound: HBM. Each row is read and written once, 136 bytes a key/value head go to the cache.
 constexpr int APPEND_THREADS = 256;
-constexpr int APPEND_HEADS = 4;
+constexpr int APPEND_FEW = 8;  // blocks a SM
 
 struct AppendParams {
   const __nv_bfloat16* qkv;
@@ -247,7 +281,8 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__global__ void __launch_bounds__(APPEND_THREADS) rope_append_paged4_kernel(const AppendParams p) {
+template <int APPEND_HEADS>
+__global__ void __launch_bounds__(APPEND_THREADS, 4) rope_append_paged4_kernel(const AppendParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int l = threadIdx.x & 7;
@@ -312,12 +347,26 @@ __global__ void __launch_bounds__(APPEND_THREADS) rope_append_paged4_kernel(cons
         const __nv_bfloat16 low_b = __float2bfloat16_rn(low);  // exact: the minimum is one of the bf16 values
         const float scale = __bfloat162float(scale_b);
         uint32_t word[2] = {0u, 0u};
+        if (scale > 0x1p-100f && scale < 0x1p100f) {
+          constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which stands in the low bits
+          constexpr uint32_t ROUND_BITS = 0x4b400000u;
+          const float inv = __frcp_rn(scale);
+          word[0] = word[1] = 0u - ROUND_BITS * 0x11111111u;  // what the other bits add up to
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          // a row of equal values has scale 0 and codes 0; NaN fails the comparison and reaches the reader through the scale
-          const float n = scale > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], low), scale)), 0.0f), 15.0f) : 0.0f;
-          word[j >> 3] |= static_cast<uint32_t>(n) << (4 * (j & 7));
-          x[j] = __fadd_rn(__fmul_rn(scale, n), low);
+          for (int j = 0; j < 16; ++j) {
+            const float d = __fsub_rn(x[j], low), t = __fmul_rn(d, inv);
+            const float n = __fadd_rn(__fmaf_rn(__fmaf_rn(-t, scale, d), inv, t), ROUND);
+            word[j >> 3] += __float_as_uint(n) << (4 * (j & 7));
+            x[j] = __fmaf_rn(scale, __fsub_rn(n, ROUND), low);  // scale * code is exact: one rounding
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            // a row of equal values has scale 0 and codes 0; NaN fails the comparison and reaches the reader through the scale
+            const float n = scale > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], low), scale)), 0.0f), 15.0f) : 0.0f;
+            word[j >> 3] |= static_cast<uint32_t>(n) << (4 * (j & 7));
+            x[j] = __fadd_rn(__fmul_rn(scale, n), low);
+          }
         }
         const bool value = h >= p.q_heads + p.kv_heads;
         const int kvh = value ? h - p.q_heads - p.kv_heads : h - p.q_heads;
@@ -373,10 +422,12 @@ extern "C" int df_page_plan(const int* seq_lens_dev, const int* new_lens_dev, in
   p.rows_per_request = rows_per_request;
   p.status = reinterpret_cast<Status*>(dev_status);
   const int smem = 3 * (requests + 1) * static_cast<int>(sizeof(int));
-  cudaError_t e = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       3 * (PLAN_MAX_REQUESTS + 1) * static_cast<int>(sizeof(int)));
-  if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  const int ctas = rows > 2 * PLAN_THREADS || requests > 2 * PLAN_THREADS ? 8 : 1;
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 * 1024) {  // more than a launch has without asking
+    e = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  }
+  const int ctas = rows > 4 * PLAN_THREADS || requests > 2 * PLAN_THREADS ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, 1, 1);
   cfg.blockDim = dim3(PLAN_THREADS, 1, 1);
@@ -387,8 +438,8 @@ extern "C" int df_page_plan(const int* seq_lens_dev, const int* new_lens_dev, in
   attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1 + dependent_launch_attr(&attr[1]);
+  cfg.attrs = ctas > 1 ? attr : attr + 1;
+  cfg.numAttrs = (ctas > 1 ? 1 : 0) + dependent_launch_attr(&attr[1]);
   e = cudaLaunchKernelEx(&cfg, page_plan_kernel, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -432,8 +483,9 @@ extern "C" int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, voi
   p.page_size = page_size;
   p.num_slots = num_pages * page_size;
   p.num_positions = num_positions;
-  const long long groups = (q_heads + 2LL * kv_heads + APPEND_HEADS - 1) / APPEND_HEADS;
-  const long long blocks = (rows * groups * 8 + APPEND_THREADS - 1) / APPEND_THREADS;
+  // heads a group of eight lanes goes through: one when there are few rows
+  const long long all = q_heads + 2LL * kv_heads, few = rows * all * 8 / APPEND_THREADS <= APPEND_FEW * sms;
+  const long long groups = few ? all : (all + 1) / 2, blocks = (rows * groups * 8 + APPEND_THREADS - 1) / APPEND_THREADS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks < 16LL * sms ? blocks : 16LL * sms), 1, 1);
   cfg.blockDim = dim3(APPEND_THREADS, 1, 1);
@@ -441,7 +493,7 @@ extern "C" int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, voi
   cudaLaunchAttribute attr;
   cfg.numAttrs = dependent_launch_attr(&attr);
   cfg.attrs = &attr;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, rope_append_paged4_kernel, p);
+  const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, rope_append_paged4_kernel<1>, p) : cudaLaunchKernelEx(&cfg, rope_append_paged4_kernel<2>, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail(DF_ECUDA, "paged rope + append launch: %s", cudaGetErrorString(e));

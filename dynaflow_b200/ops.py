@@ -95,32 +95,44 @@ def _check(rc: int, what: str) -> None:
 
 def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     """The index of the CUDA device that all the tensors are on."""
-    idx = _dev_index(first)
+    idx = first.get_device()
+    if idx < 0:
+        _dev_index(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != idx:
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
     return idx
 
 
+# the handle alone: building torch's stream object takes longer than a small call's checks
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
 def _launch(idx: int, what: str, *args) -> None:
-    """Calls an entry point with the tensors' device current (launches go to the current device)."""
+    """Calls an entry point on the current stream of device ``idx``, with that device current (launches go to the current
+    device)."""
     fn = getattr(_native.load(), what)
     if torch.cuda.current_device() == idx:
-        rc = fn(*args)
+        rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(*args)
+            rc = fn(*args, _raw_stream(idx))
     if rc != 0:
         _check(rc, what)
 
 
+def _status_ptr(idx: int) -> int:
+    st = _status.get(idx)
+    return (status_block(idx) if st is None else st).data_ptr()
+
+
 def _require_int32(name: str, t: torch.Tensor, *shape: int) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _require_bf16_2d(name: str, t: torch.Tensor) -> None:
-    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.stride(1) != 1:
+    if t.dtype is not torch.bfloat16 or t.dim() != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} must be a 2-D bf16 tensor with unit inner stride, got "
                          f"{t.dtype} {tuple(t.shape)} strides {t.stride()}")
 
@@ -372,7 +384,7 @@ def paged4_cache(num_pages: int, kv_heads: int, page_size: int, device: torch.de
 
 
 def _require_paged4(cache: torch.Tensor, page_size: int) -> None:
-    if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or page_size <= 0 \
+    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or page_size <= 0 \
             or page_size % PAGE_GRANULE or cache.shape[2] != page_size * PAGED4_TOKEN_BYTES:
         raise ValueError(f"expected a contiguous uint8 cache [pages, kv_heads, page_size * {PAGED4_TOKEN_BYTES}], page_size a "
                          f"multiple of {PAGE_GRANULE}; got {cache.dtype} {tuple(cache.shape)} and page_size {page_size}")
@@ -394,10 +406,11 @@ def page_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.
     _require_int32("seq_lens", seq_lens, B)
     _require_int32("new_lens", new_lens, B)
     _require_int32("page_counts", page_counts, B)
-    _require_int32("free_pages", free_pages, free_pages.numel())
+    num_pages = free_pages.numel()
+    _require_int32("free_pages", free_pages, num_pages)
     _require_int32("free_count", free_count, 1)
     _require_int32("row_starts", row_starts, B + 1)
-    rows = slots.numel()
+    rows = slots.shape[0]
     _require_int32("slots", slots, rows)
     _require_int32("positions", positions, rows)
     if B == 0:
@@ -405,8 +418,7 @@ def page_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.
     idx = _same_device(page_table, seq_lens, new_lens, page_counts, free_pages, free_count, row_starts, slots, positions)
     _launch(idx, "df_page_plan", seq_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), page_counts.data_ptr(),
             free_pages.data_ptr(), free_count.data_ptr(), row_starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), B,
-            max_pages, free_pages.numel(), rows, page_size, rows_per_request, status_block(page_table.device).data_ptr(),
-            _stream_ptr(page_table))
+            max_pages, num_pages, rows, page_size, rows_per_request, _status_ptr(idx))
 
 
 def rope_angles(num_positions: int, theta: float, device: torch.device | str = "cuda") -> torch.Tensor:
@@ -425,12 +437,16 @@ def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.
     Rows with a slot or position out of range are padding: left as they are in ``out``. ``angles`` from ``rope_angles``."""
     _require_bf16_2d("qkv", qkv)
     _require_paged4(cache, page_size)
-    out = qkv if out is None else out
-    if out is not qkv:
+    rows, cols = qkv.shape
+    if out is None:
+        out = qkv
+    elif out is not qkv:
         _require_bf16_2d("out", out)
-    rows = qkv.shape[0]
-    if qkv.shape[1] != (q_heads + 2 * kv_heads) * 128 or tuple(out.shape) != tuple(qkv.shape) or cache.shape[1] != kv_heads:
-        raise ValueError("expected qkv and out [rows, (q_heads + 2 kv_heads) * 128] and a cache of kv_heads heads")
+        if out.shape != (rows, cols):
+            raise ValueError(f"out must be {(rows, cols)}, got {tuple(out.shape)}")
+    num_pages, heads, _ = cache.shape
+    if cols != (q_heads + 2 * kv_heads) * 128 or heads != kv_heads:
+        raise ValueError("expected qkv [rows, (q_heads + 2 kv_heads) * 128] and a cache of kv_heads heads")
     if angles.dtype != torch.float32 or angles.dim() != 2 or angles.shape[1] != 128 or not angles.is_contiguous():
         raise ValueError("angles must be a contiguous fp32 tensor [positions, 128]")
     _require_int32("positions", positions, rows)
@@ -439,8 +455,8 @@ def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.
     if rows == 0:
         return out
     _launch(idx, "df_rope_append_paged4_bf16", qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), positions.data_ptr(),
-            slots.data_ptr(), angles.data_ptr(), angles.shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), cache.shape[0],
-            page_size, _stream_ptr(qkv))
+            slots.data_ptr(), angles.data_ptr(), angles.shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), num_pages,
+            page_size)
     return out
 
 
@@ -468,8 +484,8 @@ def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     _require_paged4(cache, page_size)
     hd = 128
     rows, cols = q.shape
-    kv_heads = cache.shape[1]
-    if cols == 0 or cols % (hd * kv_heads) or tuple(out.shape) != (rows, cols):
+    num_pages, kv_heads, _ = cache.shape
+    if cols == 0 or cols % (hd * kv_heads) or out.shape != (rows, cols):
         raise ValueError("expected q/out [rows, Hq * 128], Hq a multiple of the cache's heads")
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be [requests, max_pages], got {tuple(page_table.shape)}")
@@ -490,9 +506,9 @@ def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
         return out
     _launch(idx, "df_attention_paged4_bf16", q.data_ptr(), q.stride(0), cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
             None if row_starts is None else row_starts.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
-            out.data_ptr(), out.stride(0), rows, B, max_pages, cache.shape[0], page_size, cols // hd, kv_heads, hd, max_new,
+            out.data_ptr(), out.stride(0), rows, B, max_pages, num_pages, page_size, cols // hd, kv_heads, hd, max_new,
             hd ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), max_ctas,
-            status_block(q.device).data_ptr(), _stream_ptr(q))
+            _status_ptr(idx))
     return out
 
 
@@ -521,7 +537,7 @@ def _require_logits(logits: torch.Tensor, ids: torch.Tensor) -> tuple[int, int]:
         raise ValueError(f"logits must be 2-D bf16 or fp32 with unit inner stride, got {logits.dtype} {tuple(logits.shape)} "
                          f"strides {logits.stride()}")
     rows, vocab = logits.shape
-    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (rows,) or not ids.is_contiguous():
+    if ids.dtype not in (torch.int32, torch.int64) or ids.shape != (rows,) or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 or int64 tensor of {rows} entries, got {ids.dtype} {tuple(ids.shape)}")
     return rows, vocab
 
@@ -530,7 +546,7 @@ def _require_logprobs_out(out: tuple[torch.Tensor, ...], rows: int, top: int) ->
     lp, ent, tid, tlp = out
     for name, t, dtype, shape in (("logprob", lp, torch.float32, (rows,)), ("entropy", ent, torch.float32, (rows,)),
                                   ("top_ids", tid, torch.int32, (rows, top)), ("top_logprobs", tlp, torch.float32, (rows, top))):
-        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -552,7 +568,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out
     lp, ent, tid, tlp = out
     _launch(idx, "df_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
             ids.element_size(), rows, vocab, top, lp.data_ptr(), ent.data_ptr(), tid.data_ptr(), tlp.data_ptr(),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_ptr(logits))
+            workspace.data_ptr(), workspace.nbytes)
     return out
 
 
@@ -576,7 +592,7 @@ def token_logprobs_shard(logits: torch.Tensor, ids: torch.Tensor, vocab_start: i
         return record
     _launch(idx, "df_token_logprobs_shard", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
             ids.element_size(), rows, vocab, vocab_start, top, record.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream_ptr(logits))
+            workspace.numel() * workspace.element_size())
     return record
 
 
@@ -592,5 +608,5 @@ def token_logprobs_join(records: torch.Tensor, parts: int, rows: int, top: int, 
     idx = _same_device(records, *out)
     lp, ent, tid, tlp = out
     _launch(idx, "df_token_logprobs_join", records.data_ptr(), parts, rows, top, lp.data_ptr(), ent.data_ptr(), tid.data_ptr(),
-            tlp.data_ptr(), _stream_ptr(records))
+            tlp.data_ptr())
     return out
