@@ -26,6 +26,7 @@ import torch
 
 from . import _native, ops
 from .comm import MulticastComm, PeerComm, add_rmsnorm
+from .paged import PagedKVCache4
 
 
 @dataclasses.dataclass
@@ -102,20 +103,26 @@ class TensorParallelDecoder:
         self.comm = comm_cls(rank, world, max_rows, s.hidden, slots=n, n_ctas=n_ctas, device=dev) if world > 1 else None
         self.gemm_max_ctas = gemm_max_ctas                    # CTAs the GEMMs may use (0 = one per SM)
         self.launch_count = 0
+        self.paged: PagedKVCache4 | None = None               # init_decode_paged: the cache in pages of 4-bit codes
+        self._prefill_paged = False
 
     # ------------------------------------------------------------------ pieces
     def _partial(self, mb: int, rows: int) -> torch.Tensor:
         return self.comm.partial(mb, rows) if self.comm is not None else self.partial_local[mb][:rows]
 
-    def _attention_half(self, layer: dict, x: torch.Tensor, mb: int, batch: int, seq: int, pos: torch.Tensor) -> None:
+    def _attention_half(self, layer: dict, x: torch.Tensor, mb: int, batch: int, seq: int, pos: torch.Tensor, li: int = 0,
+                        first_row: int = 0) -> None:
         s = self.s
         rows = batch * seq
         qkv = self.qkv[mb][:rows]
         ops.gemm_bf16(x, layer["wqkv"], out=qkv, max_ctas=self.gemm_max_ctas)
-        rc = self.lib.df_rope_bf16(qkv.data_ptr(), pos.data_ptr(), rows, self.qh + self.kvh, s.head_dim, qkv.stride(0),
-                                   s.rope_theta, torch.cuda.current_stream(self.device).cuda_stream)
-        if rc != 0:
-            raise RuntimeError(_native.last_error())
+        if self._prefill_paged:      # the keys and values come back as the cache holds them: what later steps will see
+            self.paged.append(li, qkv, self.qh, first_row)
+        else:
+            rc = self.lib.df_rope_bf16(qkv.data_ptr(), pos.data_ptr(), rows, self.qh + self.kvh, s.head_dim, qkv.stride(0),
+                                       s.rope_theta, torch.cuda.current_stream(self.device).cuda_stream)
+            if rc != 0:
+                raise RuntimeError(_native.last_error())
         attn = self.attn_out[mb][:rows]
         ops.attention_prefill(qkv[:, :self.q_cols], qkv[:, self.q_cols:self.q_cols + self.kv_cols],
                               qkv[:, self.q_cols + self.kv_cols:], attn, batch=batch, seq_len=seq,
@@ -195,7 +202,7 @@ class TensorParallelDecoder:
                     main.wait_event(done[mb])
                 b, rows = rows_of[mb]
                 if not skip_compute:
-                    self._attention_half(layer, xs[mb], mb, b, seq, pos[:rows])
+                    self._attention_half(layer, xs[mb], mb, b, seq, pos[:rows], li, cuts[mb] * seq)
                 reduce_after(mb, layer["norm2"])
             nxt = self.layers[li + 1]["norm1"] if li + 1 < len(self.layers) else self.final_norm
             for mb in range(n):
@@ -215,9 +222,8 @@ class TensorParallelDecoder:
         ``fill_seed`` (``None``: zeros), the sequence lengths (every sequence holds ``context_len``
         keys AFTER the new token has been appended), and the split-KV workspace."""
         s, dev = self.s, self.device
-        n = min(self.micro_batches, batch)
-        self.d_batch, self.d_max_len = batch, max_len
-        self.d_cuts = [batch * i // n for i in range(n + 1)]
+        self._init_decode_rows(batch, max_len, context_len)
+        self.paged = None
         gen = torch.Generator(device=dev).manual_seed(fill_seed if fill_seed is not None else 0)
         shape = (s.layers, batch, max_len, self.kv_cols)
         if fill_seed is None:
@@ -229,9 +235,17 @@ class TensorParallelDecoder:
             for li in range(s.layers):           # layer by layer: no fp32 copy of the whole cache
                 self.k_cache[li].copy_(torch.randn(shape[1:], generator=gen, device=dev))
                 self.v_cache[li].copy_(torch.randn(shape[1:], generator=gen, device=dev))
+        rows = max(self.d_cuts[i + 1] - self.d_cuts[i] for i in range(len(self.d_cuts) - 1))
+        self.attn_ws = [ops.attention_decode_workspace(rows, self.qh, self.kvh, max_len, dev) for _ in range(len(self.d_cuts) - 1)]
+
+    def _init_decode_rows(self, batch: int, max_len: int, context_len: int) -> None:
+        """What a decode step needs whatever its cache: micro-batches, sequence lengths, streams, logits."""
+        s, dev = self.s, self.device
+        n = min(self.micro_batches, batch)
+        self.d_batch, self.d_max_len = batch, max_len
+        self.d_cuts = [batch * i // n for i in range(n + 1)]
         self.seq_lens = torch.full((batch,), context_len, dtype=torch.int32, device=dev)
         rows = max(self.d_cuts[i + 1] - self.d_cuts[i] for i in range(n))
-        self.attn_ws = [ops.attention_decode_workspace(rows, self.qh, self.kvh, max_len, dev) for _ in range(n)]
         self.decode_streams = [torch.cuda.Stream(device=dev) for _ in range(max(n - 1, 0))]
         # One compute stream per micro-batch pays without reductions (one GPU: 6.02 -> 5.17 ms on one rank's share of the
         # 8-rank step, the projections of one micro-batch run beside the attention of the other). With reductions the
@@ -242,6 +256,35 @@ class TensorParallelDecoder:
         self.lm_head_shard = self.lm_head[self.rank * per:(self.rank + 1) * per].contiguous()
         self.logits = [torch.empty(rows, per, dtype=torch.bfloat16, device=dev) for _ in range(n)]
 
+    def init_decode_paged(self, batch: int, max_len: int, *, page_size: int = 64, num_pages: int | None = None) -> None:
+        """The same for a cache in pages of 4-bit codes: ``num_pages`` pages a layer (default: room for ``batch`` sequences of
+        ``max_len``). Every sequence is empty (``seq_lens`` 0); ``prefill_paged`` brings prompts in, and before a ``decode_step``
+        the caller adds the new token to ``seq_lens`` (``seq_lens[b] = 0`` ends a sequence: its pages return to the pool and
+        its row's logits mean nothing)."""
+        dev = self.device
+        self._init_decode_rows(batch, max_len, 0)
+        n = len(self.d_cuts) - 1
+        if num_pages is None:
+            num_pages = batch * -(-max_len // page_size)
+        self.paged = PagedKVCache4(self.s.layers, self.kvh, num_pages=num_pages, page_size=page_size, max_requests=batch, max_len=max_len,
+                                   max_rows=max(batch, n * self.max_rows), rope_theta=self.s.rope_theta, device=dev)
+        self.new_lens = torch.ones(batch, dtype=torch.int32, device=dev)
+        self.attn_ws = [ops.attention_paged4_workspace(max(self.d_cuts[i + 1] - self.d_cuts[i], 1), self.qh, self.kvh, 1, dev) for i in range(n)]
+
+    def prefill_paged(self, ids: torch.Tensor) -> torch.Tensor:
+        """Prompts ``ids [batch, seq]`` into the empty paged cache: ``forward`` with the keys and values of every layer quantised
+        into their pages (and attended to as they are held there). Returns the hidden states; ``seq_lens`` becomes ``seq``."""
+        batch, seq = ids.shape
+        if self.paged is None or batch != self.d_batch or seq > self.d_max_len or batch * seq > self.paged.slots.shape[0]:
+            raise ValueError("prefill_paged needs init_decode_paged for this batch, and rows for all of its tokens")
+        self.seq_lens.fill_(seq)
+        self.paged.plan(self.seq_lens, torch.full_like(self.seq_lens, seq), rows_per_request=seq)
+        self._prefill_paged = True
+        try:
+            return self.forward(ids)
+        finally:
+            self._prefill_paged = False
+
     def _attention_half_decode(self, li: int, layer: dict, x: torch.Tensor, mb: int) -> None:
         """qkv projection, RoPE at the sequences' last positions, the new keys and values into the
         cache, split-KV attention over the cache, output projection into the partial buffer."""
@@ -250,11 +293,15 @@ class TensorParallelDecoder:
         rows = hi - lo
         qkv = self.qkv[mb][:rows]
         ops.gemm_bf16(x, layer["wqkv"], out=qkv, max_ctas=self.gemm_max_ctas)
-        kc, vc = self.k_cache[li, lo:hi], self.v_cache[li, lo:hi]
-        ops.rope_append(qkv, self.seq_lens[lo:hi], self.qh, self.kvh, kc, vc, s.rope_theta)
         attn = self.attn_out[mb][:rows]
-        ops.attention_decode(qkv[:, :self.q_cols], kc, vc, self.seq_lens[lo:hi], attn, self.attn_ws[mb],
-                             max_ctas=self.gemm_max_ctas)
+        if self.paged is not None:
+            self.paged.append(li, qkv, self.qh, lo)
+            self.paged.attend(li, qkv[:, :self.q_cols], attn, self.attn_ws[mb], self.seq_lens[lo:hi], lo, max_ctas=self.gemm_max_ctas)
+        else:
+            kc, vc = self.k_cache[li, lo:hi], self.v_cache[li, lo:hi]
+            ops.rope_append(qkv, self.seq_lens[lo:hi], self.qh, self.kvh, kc, vc, s.rope_theta)
+            ops.attention_decode(qkv[:, :self.q_cols], kc, vc, self.seq_lens[lo:hi], attn, self.attn_ws[mb],
+                                 max_ctas=self.gemm_max_ctas)
         ops.gemm_bf16(attn, layer["wo"], out=self._partial(mb, rows), max_ctas=self.gemm_max_ctas)
         self.launch_count += 4
 
@@ -268,6 +315,8 @@ class TensorParallelDecoder:
         n = len(self.d_cuts) - 1
         main = torch.cuda.current_stream(self.device)
         comm_stream = self.comm.stream if self.comm is not None else main
+        if self.paged is not None:       # one row a sequence; the tables serve every layer and micro-batch
+            self.paged.plan(self.seq_lens, self.new_lens, rows_per_request=1)
         # one compute stream per micro-batch (``decode_streams_per_micro_batch``): the chains of the micro-batches only
         # meet in the communication stream, so the latency-bound projections of one run beside the attention of the other
         cs = [main] + [self.decode_streams[i] if self.decode_streams_per_micro_batch else main for i in range(n - 1)]
@@ -361,6 +410,24 @@ class TensorParallelDecoder:
                 logits = self.decode_step(ids, **kw)
         torch.cuda.current_stream(self.device).wait_stream(side)
         return graph.replay, logits
+
+    def token_logprobs(self, logits: list[torch.Tensor], ids: torch.Tensor, top: int = 0) -> tuple[torch.Tensor, ...]:
+        """``(logprob, entropy, top_ids, top_logprobs)`` of a decode step's logits (``ops.token_logprobs``) for the tokens ``ids
+        [batch]``; with ``top >= 1`` ``top_ids[:, 0]`` is the greedy next token. The vocabulary may be split over the ranks: each
+        reduces its part to a record, the records are all-gathered and joined (every rank gets the results)."""
+        parts = []
+        for mb, lg in enumerate(logits):
+            chosen = ids[self.d_cuts[mb]:self.d_cuts[mb + 1]]
+            if self.world == 1:
+                parts.append(ops.token_logprobs(lg, chosen, top))
+                continue
+            rows, per = lg.shape
+            record = ops.token_logprobs_shard(lg, chosen, self.rank * per, top, ops.token_logprobs_record(rows, top, lg.device),
+                                              ops.token_logprobs_workspace(rows, per, top, lg.device))
+            records = record.new_empty(self.world * record.numel())
+            torch.distributed.all_gather_into_tensor(records, record)
+            parts.append(ops.token_logprobs_join(records, self.world, rows, top))
+        return tuple(torch.cat(p) for p in zip(*parts))
 
     def logits_last_token(self, hidden: torch.Tensor, batch: int, seq: int) -> torch.Tensor:
         """Prefill only needs the logits of each request's last token."""
