@@ -126,9 +126,25 @@ def _status_ptr(idx: int) -> int:
     return (status_block(idx) if st is None else st).data_ptr()
 
 
-def _require_int32(name: str, t: torch.Tensor, *shape: int) -> None:
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _int32(t: torch.Tensor, shape: tuple[int, ...]) -> bool:
+    return t.dtype is _I32 and t.shape == shape and t.is_contiguous()
+
+
+def _require_int32(*named: tuple[str, torch.Tensor, tuple[int, ...]]) -> None:
+    for name, t, shape in named:
+        if not _int32(t, shape):
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _row_stride(name: str, t: torch.Tensor) -> int:
+    """Of a 2-D bf16 tensor with unit inner stride."""
+    stride = t.stride()
+    if t.dtype is not _BF16 or len(stride) != 2 or stride[1] != 1:
+        _require_bf16_2d(name, t)
+    return stride[0]
 
 
 def _require_bf16_2d(name: str, t: torch.Tensor) -> None:
@@ -383,11 +399,14 @@ def paged4_cache(num_pages: int, kv_heads: int, page_size: int, device: torch.de
     return torch.empty(num_pages, kv_heads, page_size * PAGED4_TOKEN_BYTES, dtype=torch.uint8, device=device)
 
 
-def _require_paged4(cache: torch.Tensor, page_size: int) -> None:
-    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or page_size <= 0 \
-            or page_size % PAGE_GRANULE or cache.shape[2] != page_size * PAGED4_TOKEN_BYTES:
+def _paged4_shape(cache: torch.Tensor, page_size: int) -> tuple[int, int]:
+    """Pages and key/value heads of a cache."""
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or not cache.is_contiguous() or page_size <= 0 or page_size % PAGE_GRANULE \
+            or shape[2] != page_size * PAGED4_TOKEN_BYTES:
         raise ValueError(f"expected a contiguous uint8 cache [pages, kv_heads, page_size * {PAGED4_TOKEN_BYTES}], page_size a "
-                         f"multiple of {PAGE_GRANULE}; got {cache.dtype} {tuple(cache.shape)} and page_size {page_size}")
+                         f"multiple of {PAGE_GRANULE}; got {cache.dtype} {tuple(shape)} and page_size {page_size}")
+    return shape[0], shape[1]
 
 
 def page_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.Tensor, page_counts: torch.Tensor,
@@ -401,18 +420,15 @@ def page_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torch.
     Too few free pages, a full table row or too few rows are reported by ``check_status``."""
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be [requests, max_pages], got {tuple(page_table.shape)}")
-    B, max_pages = page_table.shape
-    _require_int32("page_table", page_table, B, max_pages)
-    _require_int32("seq_lens", seq_lens, B)
-    _require_int32("new_lens", new_lens, B)
-    _require_int32("page_counts", page_counts, B)
-    num_pages = free_pages.numel()
-    _require_int32("free_pages", free_pages, num_pages)
-    _require_int32("free_count", free_count, 1)
-    _require_int32("row_starts", row_starts, B + 1)
-    rows = slots.shape[0]
-    _require_int32("slots", slots, rows)
-    _require_int32("positions", positions, rows)
+    B, max_pages = table = tuple(page_table.shape)
+    num_pages, rows = free_pages.numel(), slots.numel()
+    one, per_row = (B,), (rows,)
+    if not (_int32(page_table, table) and _int32(seq_lens, one) and _int32(new_lens, one) and _int32(page_counts, one)
+            and _int32(free_pages, (num_pages,)) and _int32(free_count, (1,)) and _int32(row_starts, (B + 1,))
+            and _int32(slots, per_row) and _int32(positions, per_row)):
+        _require_int32(("page_table", page_table, table), ("seq_lens", seq_lens, one), ("new_lens", new_lens, one),
+                       ("page_counts", page_counts, one), ("free_pages", free_pages, (num_pages,)), ("free_count", free_count, (1,)),
+                       ("row_starts", row_starts, (B + 1,)), ("slots", slots, per_row), ("positions", positions, per_row))
     if B == 0:
         raise ValueError("page_plan needs at least one request")
     idx = _same_device(page_table, seq_lens, new_lens, page_counts, free_pages, free_count, row_starts, slots, positions)
@@ -435,28 +451,27 @@ def rope_append_paged4(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.
     quantised into the ``slots`` of a paged 4-bit cache, one launch. ``out`` (default: in place) receives the rotated queries,
     and keys and values as the cache stands for them, so that attention over these rows sees what later steps will see.
     Rows with a slot or position out of range are padding: left as they are in ``out``. ``angles`` from ``rope_angles``."""
-    _require_bf16_2d("qkv", qkv)
-    _require_paged4(cache, page_size)
-    rows, cols = qkv.shape
+    ld = _row_stride("qkv", qkv)
+    num_pages, heads = _paged4_shape(cache, page_size)
+    rows, cols = shape = qkv.shape
     if out is None:
-        out = qkv
-    elif out is not qkv:
-        _require_bf16_2d("out", out)
-        if out.shape != (rows, cols):
+        out, ld_out = qkv, ld
+    else:
+        ld_out = _row_stride("out", out)
+        if out.shape != shape:
             raise ValueError(f"out must be {(rows, cols)}, got {tuple(out.shape)}")
-    num_pages, heads, _ = cache.shape
     if cols != (q_heads + 2 * kv_heads) * 128 or heads != kv_heads:
         raise ValueError("expected qkv [rows, (q_heads + 2 kv_heads) * 128] and a cache of kv_heads heads")
-    if angles.dtype != torch.float32 or angles.dim() != 2 or angles.shape[1] != 128 or not angles.is_contiguous():
+    angle_shape, per_row = angles.shape, (rows,)
+    if angles.dtype is not torch.float32 or len(angle_shape) != 2 or angle_shape[1] != 128 or not angles.is_contiguous():
         raise ValueError("angles must be a contiguous fp32 tensor [positions, 128]")
-    _require_int32("positions", positions, rows)
-    _require_int32("slots", slots, rows)
+    if not (_int32(positions, per_row) and _int32(slots, per_row)):
+        _require_int32(("positions", positions, per_row), ("slots", slots, per_row))
     idx = _same_device(qkv, positions, slots, angles, cache, out)
     if rows == 0:
         return out
-    _launch(idx, "df_rope_append_paged4_bf16", qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), positions.data_ptr(),
-            slots.data_ptr(), angles.data_ptr(), angles.shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), num_pages,
-            page_size)
+    _launch(idx, "df_rope_append_paged4_bf16", qkv.data_ptr(), ld, out.data_ptr(), ld_out, positions.data_ptr(), slots.data_ptr(),
+            angles.data_ptr(), angle_shape[0], rows, q_heads, kv_heads, 128, cache.data_ptr(), num_pages, page_size)
     return out
 
 
@@ -479,36 +494,32 @@ def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     row ``b`` is request ``b``'s one new token; with ``row_starts [B + 1]`` and ``new_lens [B]`` (from ``page_plan``) request ``b``
     has rows ``row_starts[b] ...``, at most ``max_new``, causal among themselves. Rows of no request keep what they held, a row
     without keys is zeros."""
-    _require_bf16_2d("q", q)
-    _require_bf16_2d("out", out)
-    _require_paged4(cache, page_size)
-    hd = 128
-    rows, cols = q.shape
-    num_pages, kv_heads, _ = cache.shape
-    if cols == 0 or cols % (hd * kv_heads) or out.shape != (rows, cols):
+    ld_q, ld_out = _row_stride("q", q), _row_stride("out", out)
+    num_pages, kv_heads = _paged4_shape(cache, page_size)
+    rows, cols = shape = q.shape
+    if cols == 0 or cols % (128 * kv_heads) or out.shape != shape:
         raise ValueError("expected q/out [rows, Hq * 128], Hq a multiple of the cache's heads")
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be [requests, max_pages], got {tuple(page_table.shape)}")
-    B, max_pages = page_table.shape
-    _require_int32("page_table", page_table, B, max_pages)
-    _require_int32("seq_lens", seq_lens, B)
-    if (row_starts is None) != (new_lens is None):
-        raise ValueError("row_starts and new_lens come together")
-    if new_lens is not None:
-        _require_int32("row_starts", row_starts, B + 1)
-        _require_int32("new_lens", new_lens, B)
+    B, max_pages = table = tuple(page_table.shape)
+    if not (_int32(page_table, table) and _int32(seq_lens, (B,))):
+        _require_int32(("page_table", page_table, table), ("seq_lens", seq_lens, (B,)))
+    starts = lens = None
+    if row_starts is not None or new_lens is not None:
+        if row_starts is None or new_lens is None:
+            raise ValueError("row_starts and new_lens come together")
+        _require_int32(("row_starts", row_starts, (B + 1,)), ("new_lens", new_lens, (B,)))
+        starts, lens = row_starts.data_ptr(), new_lens.data_ptr()
     elif max_new != 1 or rows < B:
         raise ValueError("without new_lens every request has one row: max_new must be 1, q at least as many rows as requests")
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor")
     idx = _same_device(q, cache, page_table, seq_lens, out, workspace, row_starts, new_lens)
     if rows == 0 or B == 0:
         return out
-    _launch(idx, "df_attention_paged4_bf16", q.data_ptr(), q.stride(0), cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
-            None if row_starts is None else row_starts.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
-            out.data_ptr(), out.stride(0), rows, B, max_pages, num_pages, page_size, cols // hd, kv_heads, hd, max_new,
-            hd ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), max_ctas,
-            _status_ptr(idx))
+    _launch(idx, "df_attention_paged4_bf16", q.data_ptr(), ld_q, cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), starts,
+            lens, out.data_ptr(), ld_out, rows, B, max_pages, num_pages, page_size, cols // 128, kv_heads, 128, max_new,
+            128 ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes, max_ctas, _status_ptr(idx))
     return out
 
 
@@ -532,20 +543,21 @@ def token_logprobs_workspace(rows: int, vocab: int, top: int, device: torch.devi
     return torch.empty(need, dtype=torch.uint8, device=device)
 
 
-def _require_logits(logits: torch.Tensor, ids: torch.Tensor) -> tuple[int, int]:
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
-        raise ValueError(f"logits must be 2-D bf16 or fp32 with unit inner stride, got {logits.dtype} {tuple(logits.shape)} "
-                         f"strides {logits.stride()}")
+def _require_logits(logits: torch.Tensor, ids: torch.Tensor) -> tuple[int, int, int, bool]:
+    """Rows, vocabulary, row stride, and whether the logits are fp32."""
+    stride, dtype = logits.stride(), logits.dtype
+    if len(stride) != 2 or (dtype is not _BF16 and dtype is not torch.float32) or stride[1] != 1:
+        raise ValueError(f"logits must be 2-D bf16 or fp32 with unit inner stride, got {dtype} {tuple(logits.shape)} strides {stride}")
     rows, vocab = logits.shape
-    if ids.dtype not in (torch.int32, torch.int64) or ids.shape != (rows,) or not ids.is_contiguous():
+    if (ids.dtype is not torch.int64 and ids.dtype is not _I32) or ids.shape != (rows,) or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 or int64 tensor of {rows} entries, got {ids.dtype} {tuple(ids.shape)}")
-    return rows, vocab
+    return rows, vocab, stride[0], dtype is not _BF16
 
 
 def _require_logprobs_out(out: tuple[torch.Tensor, ...], rows: int, top: int) -> None:
     lp, ent, tid, tlp = out
     for name, t, dtype, shape in (("logprob", lp, torch.float32, (rows,)), ("entropy", ent, torch.float32, (rows,)),
-                                  ("top_ids", tid, torch.int32, (rows, top)), ("top_logprobs", tlp, torch.float32, (rows, top))):
+                                  ("top_ids", tid, _I32, (rows, top)), ("top_logprobs", tlp, torch.float32, (rows, top))):
         if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
@@ -555,7 +567,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out
     """``(logprob, entropy, top_ids, top_logprobs)`` of ``logits [rows, vocab]`` (bf16 or fp32, any row stride): the log
     probability of ``ids [rows]``, the entropy (nats), and the ``top`` most likely tokens, largest first, of equal logits the
     lower index first. Forbidden tokens are ``-inf``; a row of nothing else has log probabilities ``-inf`` and entropy 0."""
-    rows, vocab = _require_logits(logits, ids)
+    rows, vocab, ld, fp32 = _require_logits(logits, ids)
     if out is None:
         out = token_logprobs_out(rows, top, logits.device)
     else:
@@ -566,7 +578,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out
     if rows == 0:
         return out
     lp, ent, tid, tlp = out
-    _launch(idx, "df_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
+    _launch(idx, "df_token_logprobs", logits.data_ptr(), fp32, ld, ids.data_ptr(),
             ids.element_size(), rows, vocab, top, lp.data_ptr(), ent.data_ptr(), tid.data_ptr(), tlp.data_ptr(),
             workspace.data_ptr(), workspace.nbytes)
     return out
@@ -584,13 +596,13 @@ def token_logprobs_shard(logits: torch.Tensor, ids: torch.Tensor, vocab_start: i
                          workspace: torch.Tensor) -> torch.Tensor:
     """This rank's part of ``token_logprobs`` when ``logits`` are tokens ``vocab_start ...`` of a split vocabulary (``ids`` are of
     the whole one). The ranks' records, all-gathered in rank order, give the results with ``token_logprobs_join``."""
-    rows, vocab = _require_logits(logits, ids)
+    rows, vocab, ld, fp32 = _require_logits(logits, ids)
     if record.dtype != torch.uint8 or not record.is_contiguous() or record.numel() < int(_native.load().df_token_logprobs_record_bytes(rows, top)):
         raise ValueError("record must be a contiguous uint8 tensor from token_logprobs_record")
     idx = _same_device(logits, ids, record, workspace)
     if rows == 0:
         return record
-    _launch(idx, "df_token_logprobs_shard", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), ids.data_ptr(),
+    _launch(idx, "df_token_logprobs_shard", logits.data_ptr(), fp32, ld, ids.data_ptr(),
             ids.element_size(), rows, vocab, vocab_start, top, record.data_ptr(), workspace.data_ptr(),
             workspace.numel() * workspace.element_size())
     return record
