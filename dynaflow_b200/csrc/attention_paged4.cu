@@ -199,7 +199,8 @@ struct AttnShared {
   Ends ends[WARPS];
   int order[WARPS];                              // the warps that have tiles
   uint32_t abort;
-  int joins[2];                                  // whether this CTA joins the parts of its first / last segment
+  unsigned cost, parts, whole;                   // the cut: cost of the list, CTAs with work, whether segments stay whole
+  int2 joins[2];                                 // first CTA and number of the parts of its first / last segment that this CTA joins
   static_assert(STAGES * TILE_BYTES >= COLS * PARTIAL_FLOATS * 4, "a partial result fits into the ring");
 };
 
@@ -271,8 +272,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   uint2* prefix = in_smem ? sm.prefix : p.prefix;
   uint2 all{0, 0};
   unsigned longest = 0;  // tiles
-  for (int b0 = 0; b0 < p.requests; b0 += THREADS) {
-    const int b = b0 + threadIdx.x;
+  auto take_in = [&](int b) {  // a request's tiles and segments
     uint2 v{0, 0};
     if (b < p.requests) {
       const Weight w = load_weight<COLS>(p, b);
@@ -281,83 +281,123 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       if (in_smem) sm.lens[b] = make_int2(w.len, w.fresh);
       if (w.blocks > 0) longest = max(longest, static_cast<unsigned>(w.tiles));
     }
-    uint2 inc = v;
+    return v;
+  };
+  auto scan = [&](uint2 v) {  // sums over this lane and those before it
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned ux = __shfl_up_sync(0xffffffffu, inc.x, o), uy = __shfl_up_sync(0xffffffffu, inc.y, o);
+      const unsigned ux = __shfl_up_sync(0xffffffffu, v.x, o), uy = __shfl_up_sync(0xffffffffu, v.y, o);
       if (lane >= o) {
-        inc.x += ux;
-        inc.y += uy;
+        v.x += ux;
+        v.y += uy;
       }
     }
-    if (b0 > 0) __syncthreads();
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    if (lane == 31) {
-      sm.warp_sum[warp] = inc;
-      sm.warp_longest[warp] = longest;
+    return v;
+  };
+  if (p.requests <= 4 * 32) {  // one warp, four requests a lane
+    if (warp == 0) {
+      uint2 v[4], own{0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = take_in(4 * lane + i);
+        own.x += v[i].x;
+        own.y += v[i].y;
+      }
+      const uint2 inc = scan(own);
+      uint2 before = make_uint2(inc.x - own.x, inc.y - own.y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * lane + i < p.requests) prefix[4 * lane + i] = before;
+        before.x += v[i].x;
+        before.y += v[i].y;
+      }
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      all = make_uint2(__shfl_sync(0xffffffffu, inc.x, 31), __shfl_sync(0xffffffffu, inc.y, 31));
+      __syncwarp();
+    }
+  } else {
+    for (int b0 = 0; b0 < p.requests; b0 += THREADS) {
+      const int b = b0 + threadIdx.x;
+      const uint2 v = take_in(b), inc = scan(v);
+      if (b0 > 0) __syncthreads();
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (lane == 31) {
+        sm.warp_sum[warp] = inc;
+        sm.warp_longest[warp] = longest;
+      }
+      __syncthreads();
+      uint2 before = all;
+      const int holding = min(WARPS, (p.requests - b0 + 31) >> 5);  // warps with a request
+      for (int i = 0; i < holding; ++i) {
+        const uint2 s = sm.warp_sum[i];
+        longest = max(longest, sm.warp_longest[i]);
+        if (i < warp) {
+          before.x += s.x;
+          before.y += s.y;
+        }
+        all.x += s.x;
+        all.y += s.y;
+      }
+      if (b < p.requests) prefix[b] = make_uint2(before.x + inc.x - v.x, before.y + inc.y - v.y);
     }
     __syncthreads();
-    uint2 before = all;
-    const int holding = min(WARPS, (p.requests - b0 + 31) >> 5);  // warps with a request
-    for (int i = 0; i < holding; ++i) {
-      const uint2 s = sm.warp_sum[i];
-      longest = max(longest, sm.warp_longest[i]);
-      if (i < warp) {
-        before.x += s.x;
-        before.y += s.y;
-      }
-      all.x += s.x;
-      all.y += s.y;
-    }
-    if (b < p.requests) prefix[b] = make_uint2(before.x + inc.x - v.x, before.y + inc.y - v.y);
   }
-  if (all.x == 0) return;
-  const unsigned cost = cost_of(all);
-  const Cut cut(cost, min(static_cast<unsigned>(gridDim.x), (cost + WARPS - 1) / WARPS));
-  // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
-  // head, on 148 CTAs: 23.2 us against 27.1 us cut evenly)
-  const unsigned per_cta = (all.y + gridDim.x - 1) / gridDim.x;
-  const bool whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
-  const unsigned parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;
-  if (blockIdx.x >= parts) return;
-  if (threadIdx.x < 2) sm.joins[threadIdx.x] = 0;
-  __syncthreads();
 
   auto weight = [&](int b) { return in_smem ? weight_of<COLS>(p, sm.lens[b].x, sm.lens[b].y) : load_weight<COLS>(p, b); };
-  // the last request for which `before` (of what lies before it) is at most x: it is not empty
-  auto find = [&](unsigned x, auto before) {
-    int lo = 0, hi = p.requests;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before(prefix[mid]) <= x) lo = mid; else hi = mid;
-    }
-    return lo;
-  };
-  // tiles that lie before a place of the list given as cost, and the request that the place is in
-  int cut_b = 0;
-  auto tiles_before = [&](unsigned at) {
-    if (at >= cost) return all.x;
-    cut_b = find(at, [](const uint2& v) { return cost_of(v); });
-    const unsigned tiles = weight(cut_b).tiles, rel = at - cost_of(prefix[cut_b]), each = tiles + SEGMENT_COST;
-    const unsigned s = rel / each, in = rel - s * each;
-    return prefix[cut_b].x + s * tiles + (in > SEGMENT_COST ? in - SEGMENT_COST : 0u);
-  };
-  auto part_start = [&](unsigned c) {
-    if (!whole) return cut.start(c);
-    const unsigned s = c * per_cta;
-    if (s >= all.y) return cost;
-    const int b = find(s, [](const uint2& v) { return v.y; });
-    return cost_of(prefix[b]) + (s - prefix[b].y) * (static_cast<unsigned>(weight(b).tiles) + SEGMENT_COST);
-  };
-  // the parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins. (Every warp has the queries of
-  // its first segment to fetch: the CTA's first segment costs nothing more.)
+  auto cut_of = [&](unsigned cost) { return Cut(cost, min(static_cast<unsigned>(gridDim.x), (cost + WARPS - 1) / WARPS)); };
   if (warp == 0) {
-    const unsigned bound = part_start(blockIdx.x + (lane & 1));
-    const unsigned at0 = __shfl_sync(0xffffffffu, bound, 0) + (whole ? SEGMENT_COST : 0u), at_n = __shfl_sync(0xffffffffu, bound, 1) - at0;
-    const unsigned cut_at = tiles_before(at0 + Cut(at_n, WARPS).start(min(lane, WARPS)));
-    if (lane <= WARPS) sm.part[lane] = make_uint2(cut_at, cut_b);
+    const unsigned cost = cost_of(all);
+    unsigned parts = 0, per_cta = 1;
+    bool whole = false;
+    if (cost > 0) {
+      const Cut cut = cut_of(cost);
+      // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
+      // head, on 148 CTAs: 23.2 us against 27.1 us cut evenly)
+      per_cta = (all.y + gridDim.x - 1) / gridDim.x;
+      whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
+      parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;
+      if (blockIdx.x < parts) {
+        // the last request for which `before` (of what lies before it) is at most x: it is not empty
+        auto find = [&](unsigned x, auto before) {
+          int lo = 0, hi = p.requests;
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (before(prefix[mid]) <= x) lo = mid; else hi = mid;
+          }
+          return lo;
+        };
+        auto part_start = [&](unsigned c) {
+          if (!whole) return cut.start(c);
+          const unsigned s = c * per_cta;
+          if (s >= all.y) return cost;
+          const int b = find(s, [](const uint2& v) { return v.y; });
+          return cost_of(prefix[b]) + (s - prefix[b].y) * (static_cast<unsigned>(weight(b).tiles) + SEGMENT_COST);
+        };
+        // The parts of this CTA's warps, cut by cost too: lane w finds where warp w's begins. (Every warp has the queries of
+        // its first segment to fetch: the CTA's first segment costs nothing more.)
+        const unsigned bound = part_start(blockIdx.x + (lane & 1));
+        const unsigned at0 = __shfl_sync(0xffffffffu, bound, 0) + (whole ? SEGMENT_COST : 0u), at_n = __shfl_sync(0xffffffffu, bound, 1) - at0;
+        const unsigned at = at0 + Cut(at_n, WARPS).start(min(lane, WARPS));
+        uint2 begin{all.x, 0u};  // tiles that lie before that place, and the request that it is in
+        if (at < cost) {
+          const int b = find(at, [](const uint2& v) { return cost_of(v); });
+          const unsigned tiles = weight(b).tiles, rel = at - cost_of(prefix[b]), each = tiles + SEGMENT_COST;
+          const unsigned s = rel / each, in = rel - s * each;
+          begin = make_uint2(prefix[b].x + s * tiles + (in > SEGMENT_COST ? in - SEGMENT_COST : 0u), static_cast<unsigned>(b));
+        }
+        if (lane <= WARPS) sm.part[lane] = begin;
+      }
+    }
+    if (lane == 0) {
+      sm.cost = cost;
+      sm.parts = parts;
+      sm.whole = whole;
+      sm.joins[0] = sm.joins[1] = make_int2(0, 0);
+    }
   }
   __syncthreads();
+  if (blockIdx.x >= sm.parts) return;
+  const bool whole = sm.whole != 0u;
   const unsigned f0 = sm.part[warp].x;
   const int count = static_cast<int>(sm.part[warp + 1].x - f0);
   int cur_b = static_cast<int>(sm.part[warp].y);  // request of the part's first tile, then of the last look-up's first
@@ -381,15 +421,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       ahead.hc = static_cast<int>(hc);
       ahead.flags = tile << 3 | (tile == 0 && n + lane > 0 ? TILE_FIRST : 0);
       const int kvh = w.blocks == 1 ? ahead.hc : ahead.hc / w.blocks;
+      int column = 2 * tile / p.page_granules, in_page = 2 * tile - column * p.page_granules;  // the length keeps it inside the table
+      const int* row = p.table + static_cast<size_t>(b) * p.max_pages;
+      const int page0 = w.len > 0 ? row[column] : -1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int granule = 2 * tile + h;
-        if (granule * GRANULE >= w.len) continue;
-        const int column = granule / p.page_granules;  // inside the table: the length is limited to what a row can hold
-        const int page = p.table[static_cast<size_t>(b) * p.max_pages + column];
+        if ((2 * tile + h) * GRANULE >= w.len) break;
+        if (h == 1 && ++in_page == p.page_granules) {
+          in_page = 0;
+          ++column;
+        }
+        const int page = h == 1 && in_page == 0 ? row[column] : page0;
         if (page >= 0 && page < p.num_pages) {
           ahead.flags |= 1 << h;
-          ahead_src[h] = p.cache + ((static_cast<size_t>(page) * p.kv_heads + kvh) * p.page_granules + (granule - column * p.page_granules)) * GRANULE_BYTES;
+          ahead_src[h] = p.cache + ((static_cast<size_t>(page) * p.kv_heads + kvh) * p.page_granules + in_page) * GRANULE_BYTES;
         }
       }
     }
@@ -670,6 +715,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         }
       }
     }
+    // with registers to spare the value fragments are on their way while the softmax works
+    constexpr bool EARLY = NT == 2;
+    uint32_t vf[2][2][4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
+    auto load_values = [&](int h, int half) { ldmatrix_x4_trans(smem_u32(st) + h * GRANULE_BYTES + (lm_off ^ (half * 32)), vf[h][half]); };
+    if (EARLY) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_values(i >> 1, i & 1);
+    }
     // ---- scores less their reference, log2
     float vs[2][2], vm[2][2];
 #pragma unroll
@@ -784,14 +837,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
       }
-      const uint32_t st_addr = smem_u32(st) + h * GRANULE_BYTES;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t v[4];  // (keys 0-7, keys 8-15) of chunk 2 half, then of chunk 2 half + 1
-        ldmatrix_x4_trans(st_addr + (lm_off ^ (half * 32)), v);
+        if (!EARLY) load_values(h, half);
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          const uint32_t x0 = v[2 * cc], x1 = v[2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+          const uint32_t x0 = vf[h][half][2 * cc], x1 = vf[h][half][2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_f16(acc[nt][4 * half + 2 * cc], code_lo(x0), code_hi(x0), code_lo(x1), code_hi(x1), pf[nt][0], pf[nt][1]);
@@ -851,9 +902,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     c.links = (c.ended ? c.start + 1 + __ffs(ends) : active) - max(c.start, 0);
     return c;
   };
-  for (int task = warp; task < chains * COLS; task += WARPS) {
-    const int local = task % COLS;
-    const Chain ch = chain_of(task / COLS);
+  const int columns = min(COLS, p.max_new * p.group);  // of a segment with queries, at most
+  for (int task = warp; task < chains * columns; task += WARPS) {
+    const int k = task / columns, local = task - k * columns;
+    const Chain ch = chain_of(k);
     const Weight w = weight(ch.b);
     int kvh, column0, row0;
     place(w, ch.b, ch.hc, kvh, column0, row0);
@@ -883,38 +935,58 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   __syncthreads();
   const Chain first = chain_of(0), last = chain_of(chains - 1);
   const bool cut0 = first.start < 0, cut1 = last.start >= 0 && !last.ended;
-  auto span = [&](const Chain& ch, int& c0, int& c1) {  // the CTAs that hold tiles of its segment
-    const unsigned tiles = weight(ch.b).tiles, at = cost_of(prefix[ch.b]) + ch.hc * (tiles + SEGMENT_COST) + SEGMENT_COST;
-    c0 = static_cast<int>(cut.part_of(at));
-    c1 = static_cast<int>(cut.part_of(at + tiles - 1));
-  };
   if (threadIdx.x < 2 && (threadIdx.x == 0 ? cut0 : cut1)) {
-    int c0, c1;
-    span(threadIdx.x == 0 ? first : last, c0, c1);
-    __threadfence();  // the parts that the other warps wrote before the barrier, too
-    if (atomicAdd(p.arrived + c0, 1) == c1 - c0) {
+    const Chain& ch = threadIdx.x == 0 ? first : last;
+    // the CTAs that hold tiles of its segment
+    const Cut cut = cut_of(sm.cost);
+    const unsigned tiles = weight(ch.b).tiles, at = cost_of(prefix[ch.b]) + ch.hc * (tiles + SEGMENT_COST) + SEGMENT_COST;
+    const int c0 = static_cast<int>(cut.part_of(at)), n = static_cast<int>(cut.part_of(at + tiles - 1)) - c0 + 1;
+    int before_me;  // releases what the other warps wrote before the barrier, acquires what the other CTAs released
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before_me) : "l"(p.arrived + c0) : "memory");
+    if (before_me == n - 1) {
       p.arrived[c0] = 0;  // nobody else comes in this launch
-      sm.joins[threadIdx.x] = 1;
+      sm.joins[threadIdx.x] = make_int2(c0, n);
     }
-    __threadfence();
   }
   __syncthreads();
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    if (sm.joins[k] == 0) continue;
+    const int c0 = sm.joins[k].x, n = sm.joins[k].y;
+    if (n == 0) continue;
     const Chain& ch = k == 0 ? first : last;
-    int c0, c1;
-    span(ch, c0, c1);
     const Weight w = weight(ch.b);
     int kvh, column0, row0;
     place(w, ch.b, ch.hc, kvh, column0, row0);
-    for (int local = warp; local < COLS; local += WARPS) {
+    // several warps a column if there are many parts; what they join lies in the rings until one of them joins that
+    const int share = n > 8 ? max(WARPS / columns, 1) : 1;
+    auto finish = [&](int local, float4 v, float sum) {
       const int c = column0 + local, j = div_small(c, p.inv_group), row = row0 + j;
-      if (j >= min(w.fresh, p.max_new) || row < 0 || row >= p.rows) continue;
-      auto link = [&](int i) -> const float* { return p.partial + ((static_cast<size_t>(c0 + i) * 2 + (i == 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS; };
+      if (j < min(w.fresh, p.max_new) && row >= 0 && row < p.rows)
+        store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+    };
+    for (int task = warp; task < columns * share; task += WARPS) {
+      const int local = task / share, q = task - local * share, i0 = n * q / share, i1 = n * (q + 1) / share;
+      if (div_small(column0 + local, p.inv_group) >= min(w.fresh, p.max_new)) continue;  // no query, no part
+      auto link = [&](int i) -> const float* { return p.partial + ((static_cast<size_t>(c0 + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS; };
       float sum, joined;
-      const float4 v = join_links(c1 - c0 + 1, link, lane, sum, joined);
-      store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+      const float4 v = join_links(i1 - i0, link, lane, sum, joined);
+      if (share == 1) {
+        finish(local, v, sum);
+      } else {
+        float* slot = reinterpret_cast<float*>(sm.ring[warp][0]);
+        *reinterpret_cast<float4*>(slot + 4 * lane) = v;
+        if (lane == 0) *reinterpret_cast<float2*>(slot + HEAD_DIM) = make_float2(joined, sum);
+      }
+    }
+    if (share > 1) {  // columns * share warps, a task each
+      __syncthreads();
+      if (warp < columns && div_small(column0 + warp, p.inv_group) < min(w.fresh, p.max_new)) {
+        auto link = [&](int i) -> const float* { return reinterpret_cast<const float*>(sm.ring[warp * share + i][0]); };
+        float sum, joined;
+        const float4 v = join_links(share, link, lane, sum, joined);
+        finish(warp, v, sum);
+      }
+      __syncthreads();
     }
   }
 }
