@@ -51,7 +51,7 @@ constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padde
 constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
 constexpr int TILE = 2 * GRANULE;             // tokens
 constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
-constexpr unsigned SEGMENT_COST = 2;          // tiles
+constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 33.9 us; 1: 39.5, 2: 34.4, 4: 33.8)
 constexpr unsigned JOIN_COST = 40;            // tiles of 8 columns a CTA does in the time that a join between CTAs takes
 constexpr int MAX_COLUMNS = 1 << 20;
 
@@ -884,68 +884,63 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   const unsigned tails = __ballot_sync(0xffffffffu, lane < active && sm.ends[sm.order[lane < active ? lane : 0]].tail_b >= 0);
   const int before = sm.ends[sm.order[0]].head_b >= 0 ? 1 : 0, chains = before + __popc(tails);
   if (chains == 0) return;
-  struct Chain {
-    int b, hc, start, links;  // start: place among the warps with work of the one whose tail it begins with, -1: the first one's head
-    bool ended;
-  };
   const unsigned ending = __ballot_sync(0xffffffffu, lane < active && sm.ends[sm.order[lane < active ? lane : 0]].head_ends != 0);
-  auto chain_of = [&](int k) {
-    Chain c;
+  // lane k has chain k: where it begins (place among the warps with work of the one with its tail, -1: the first one's
+  // head), its links, and what its rows are
+  int ch_b = 0, ch_hc = 0, ch_start = -1, ch_links = 0, ch_head = 0, ch_column0 = 0, ch_row0 = 0, ch_served = 0;
+  bool ch_ended = false;
+  if (lane < chains) {
     unsigned later = tails;
-    for (int i = before; i < k; ++i) later &= later - 1u;
-    c.start = k < before ? -1 : __ffs(later) - 1;
-    const Ends& e = sm.ends[sm.order[max(c.start, 0)]];
-    c.b = c.start < 0 ? e.head_b : e.tail_b;
-    c.hc = c.start < 0 ? e.head_hc : e.tail_hc;
-    const unsigned ends = c.start + 1 < 32 ? ending >> (c.start + 1) : 0u;  // the first of the following heads that ends
-    c.ended = ends != 0u;
-    c.links = (c.ended ? c.start + 1 + __ffs(ends) : active) - max(c.start, 0);
-    return c;
-  };
+    for (int i = before; i < lane; ++i) later &= later - 1u;
+    if (lane >= before) ch_start = __ffs(later) - 1;
+    const Ends& e = sm.ends[sm.order[max(ch_start, 0)]];
+    ch_b = ch_start < 0 ? e.head_b : e.tail_b;
+    ch_hc = ch_start < 0 ? e.head_hc : e.tail_hc;
+    const unsigned ends = ending >> (ch_start + 1);  // the first of the following heads that ends (at most 16 warps)
+    ch_ended = ends != 0u;
+    ch_links = (ch_ended ? ch_start + 1 + __ffs(ends) : active) - max(ch_start, 0);
+    const Weight w = weight(ch_b);
+    place(w, ch_b, ch_hc, ch_head, ch_column0, ch_row0);
+    ch_head *= p.group;
+    ch_served = min(w.fresh, p.max_new);
+  }
   const int columns = min(COLS, p.max_new * p.group);  // of a segment with queries, at most
   for (int task = warp; task < chains * columns; task += WARPS) {
     const int k = task / columns, local = task - k * columns;
-    const Chain ch = chain_of(k);
-    const Weight w = weight(ch.b);
-    int kvh, column0, row0;
-    place(w, ch.b, ch.hc, kvh, column0, row0);
-    const int c = column0 + local, j = div_small(c, p.inv_group), row = row0 + j;
-    if (j >= min(w.fresh, p.max_new) || row < 0 || row >= p.rows) continue;
+    const int start = __shfl_sync(0xffffffffu, ch_start, k), links = __shfl_sync(0xffffffffu, ch_links, k);
+    const int c = __shfl_sync(0xffffffffu, ch_column0, k) + local, j = div_small(c, p.inv_group);
+    const int row = __shfl_sync(0xffffffffu, ch_row0, k) + j, head = __shfl_sync(0xffffffffu, ch_head, k) + c - j * p.group;
+    const bool ended = __shfl_sync(0xffffffffu, ch_ended, k), here = j < __shfl_sync(0xffffffffu, ch_served, k);
+    if (!here || row < 0 || row >= p.rows) continue;
     auto link = [&](int i) -> const float* {
-      const int w = sm.order[max(ch.start, 0) + i];
-      const bool in_ring = (ch.start >= 0 && i == 0) || sm.ends[w].head_in_ring != 0;
+      const int w = sm.order[max(start, 0) + i];
+      const bool in_ring = (start >= 0 && i == 0) || sm.ends[w].head_in_ring != 0;
       return (in_ring ? reinterpret_cast<const float*>(sm.ring[w][0]) : p.heads + (static_cast<size_t>(blockIdx.x) * WARPS + w) * COLS * PARTIAL_FLOATS) + local * PARTIAL_FLOATS;
     };
     float sum, joined;
-    const float4 v = join_links(ch.links, link, lane, sum, joined);
-    if (ch.start >= 0 && ch.ended) {
-      store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+    const float4 v = join_links(links, link, lane, sum, joined);
+    if (start >= 0 && ended) {
+      store_row(p.out + row * p.ld_out + head * HEAD_DIM + 4 * lane, v, sum);
     } else {
-      float* slot = p.partial + ((static_cast<size_t>(blockIdx.x) * 2 + (ch.start >= 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS;
+      float* slot = p.partial + ((static_cast<size_t>(blockIdx.x) * 2 + (start >= 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS;
       *reinterpret_cast<float4*>(slot + 4 * lane) = v;
-      if (lane == 0) {
-        slot[HEAD_DIM] = joined;
-        slot[HEAD_DIM + 1] = sum;
-      }
+      if (lane == 0) *reinterpret_cast<float2*>(slot + HEAD_DIM) = make_float2(joined, sum);
     }
   }
 
   if (whole) return;
   // ---- what is cut between CTAs: the first chain if it began in an earlier CTA, the last one if it goes on
   __syncthreads();
-  const Chain first = chain_of(0), last = chain_of(chains - 1);
-  const bool cut0 = first.start < 0, cut1 = last.start >= 0 && !last.ended;
-  if (threadIdx.x < 2 && (threadIdx.x == 0 ? cut0 : cut1)) {
-    const Chain& ch = threadIdx.x == 0 ? first : last;
-    // the CTAs that hold tiles of its segment
+  if (warp == 0 && lane < chains && ((lane == 0 && ch_start < 0) || (lane == chains - 1 && ch_start >= 0 && !ch_ended))) {
+    // the CTAs that hold tiles of the segment
     const Cut cut = cut_of(sm.cost);
-    const unsigned tiles = weight(ch.b).tiles, at = cost_of(prefix[ch.b]) + ch.hc * (tiles + SEGMENT_COST) + SEGMENT_COST;
+    const unsigned tiles = weight(ch_b).tiles, at = cost_of(prefix[ch_b]) + ch_hc * (tiles + SEGMENT_COST) + SEGMENT_COST;
     const int c0 = static_cast<int>(cut.part_of(at)), n = static_cast<int>(cut.part_of(at + tiles - 1)) - c0 + 1;
     int before_me;  // releases what the other warps wrote before the barrier, acquires what the other CTAs released
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before_me) : "l"(p.arrived + c0) : "memory");
     if (before_me == n - 1) {
       p.arrived[c0] = 0;  // nobody else comes in this launch
-      sm.joins[threadIdx.x] = make_int2(c0, n);
+      sm.joins[ch_start < 0 ? 0 : 1] = make_int2(c0, n);
     }
   }
   __syncthreads();
@@ -953,20 +948,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   for (int k = 0; k < 2; ++k) {
     const int c0 = sm.joins[k].x, n = sm.joins[k].y;
     if (n == 0) continue;
-    const Chain& ch = k == 0 ? first : last;
-    const Weight w = weight(ch.b);
-    int kvh, column0, row0;
-    place(w, ch.b, ch.hc, kvh, column0, row0);
+    const int chain = k == 0 ? 0 : chains - 1;
+    const int column0 = __shfl_sync(0xffffffffu, ch_column0, chain), row0 = __shfl_sync(0xffffffffu, ch_row0, chain);
+    const int head0 = __shfl_sync(0xffffffffu, ch_head, chain), served = __shfl_sync(0xffffffffu, ch_served, chain);
     // several warps a column if there are many parts; what they join lies in the rings until one of them joins that
     const int share = n > 8 ? max(WARPS / columns, 1) : 1;
     auto finish = [&](int local, float4 v, float sum) {
       const int c = column0 + local, j = div_small(c, p.inv_group), row = row0 + j;
-      if (j < min(w.fresh, p.max_new) && row >= 0 && row < p.rows)
-        store_row(p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
+      if (j < served && row >= 0 && row < p.rows) store_row(p.out + row * p.ld_out + (head0 + c - j * p.group) * HEAD_DIM + 4 * lane, v, sum);
     };
     for (int task = warp; task < columns * share; task += WARPS) {
       const int local = task / share, q = task - local * share, i0 = n * q / share, i1 = n * (q + 1) / share;
-      if (div_small(column0 + local, p.inv_group) >= min(w.fresh, p.max_new)) continue;  // no query, no part
+      if (div_small(column0 + local, p.inv_group) >= served) continue;  // no query, no part
       auto link = [&](int i) -> const float* { return p.partial + ((static_cast<size_t>(c0 + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * COLS + local) * PARTIAL_FLOATS; };
       float sum, joined;
       const float4 v = join_links(i1 - i0, link, lane, sum, joined);
@@ -980,7 +973,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     }
     if (share > 1) {  // columns * share warps, a task each
       __syncthreads();
-      if (warp < columns && div_small(column0 + warp, p.inv_group) < min(w.fresh, p.max_new)) {
+      if (warp < columns && div_small(column0 + warp, p.inv_group) < served) {
         auto link = [&](int i) -> const float* { return reinterpret_cast<const float*>(sm.ring[warp * share + i][0]); };
         float sum, joined;
         const float4 v = join_links(share, link, lane, sum, joined);
