@@ -33,7 +33,11 @@
 // A request and head costs a warp its queries and its result as well as its tiles, so it counts SEGMENT_COST tiles
 // more when the list is cut (without: 16 requests of a few tokens among long ones make one CTA twice as long).
 //
-// Bound: HBM, 136 bytes a key and head.
+// Bound: HBM, 136 bytes a key and head: long caches stream at 6.3 TB/s (the difference between 65536 and 32768 tokens,
+// 8 requests, 8 heads: 285 MB in 45 us). Short ones are bound by what lies around that: about 5 us from the lengths
+// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 23.4 us.
+// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 74 us) a warp's chain of
+// products and softmax is longer than its share of the bytes takes, at two warps a scheduler (228 registers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     if (cost > 0) {
       const Cut cut = cut_of(cost);
       // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
-      // head, on 148 CTAs: 23.2 us against 27.1 us cut evenly)
+      // head, on 148 CTAs: 23.4 us against 26.2 us cut evenly)
       per_cta = (all.y + gridDim.x - 1) / gridDim.x;
       whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
       parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;

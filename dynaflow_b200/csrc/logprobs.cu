@@ -16,7 +16,9 @@
 // what reaches it into a list, which is ranked by comparing all pairs. If it does not fit (a great many equal logits),
 // the k largest keys are selected by bisection instead.
 //
-// Bound: HBM, each logit is read once; then the exponentials (16 a clock and SM). The next chunk is fetched while one
+// Bound: HBM, each logit is read once (2048 x 128256 bf16, sums alone: 84.8 us = 6.2 TB/s), then the exponentials (16 a
+// clock and SM). With the most likely tokens the end of a block (threshold, reading again, ranking, 6 to 8 us) is in the
+// way of few rows: 256 x 128256, 20 tokens: 25 us, sums alone 17 us. The next chunk is fetched while one
 // is worked on. When there are few rows, a row is cut into slices: up to eight are one thread-block cluster, whose
 // first CTA joins them through distributed shared memory; more of them (a very long row) leave records in the
 // workspace for a second launch, which also joins the shards of a vocabulary that is split over ranks.

@@ -29,7 +29,8 @@ namespace paged {
 //
 // What bounds it: latency. One cluster of CTAs does it all in one launch (a few KB to some hundred KB of
 // integers); every CTA repeats the prefix sums over the requests in its own shared memory, and the cluster
-// barrier separates "everyone has read the old state" from "the new state is written".
+// barrier separates "everyone has read the old state" from "the new state is written". One CTA up to 4096 rows (256
+// requests, a step and its return: 10.4 us), eight above (61 prompts, 125000 rows, and their return: 16.5 us).
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_REQUESTS = 8192;
 
@@ -237,7 +238,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanParam
 // correctly rounded d / scale (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990);
 // scales so small or large that a step could leave the normal numbers take the division itself.
 //
-// Bound: HBM. Each row is read and written once, 136 bytes a key/value head go to the cache.
+// Bound: HBM. Each row is read and written once, 136 bytes a key/value head go to the cache: 16384 rows of 32 + 2 x 8
+// heads, 429 MB in 82 us = 5.2 TB/s. Two heads a group, four blocks a SM (one head: 89 us; four, two blocks: 86 us).
+// Few rows are bound by the chain slot -> row -> angles: one head a group (256 rows: 3.5 us; two 4.1, four 4.3).
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_FEW = 8;  // blocks a SM
 
