@@ -493,7 +493,7 @@ def attention_paged4(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     ``cache [pages, Hkv, page_size * 136]``, ``page_table [B, max_pages]`` and ``seq_lens [B]`` int32. Without ``new_lens``
     row ``b`` is request ``b``'s one new token; with ``row_starts [B + 1]`` and ``new_lens [B]`` (from ``page_plan``) request ``b``
     has rows ``row_starts[b] ...``, at most ``max_new``, causal among themselves. Rows of no request keep what they held, a row
-    without keys is zeros."""
+    without keys is zeros. Lengths past what a row of the table holds are limited to that."""
     ld_q, ld_out = _row_stride("q", q), _row_stride("out", out)
     num_pages, kv_heads = _paged4_shape(cache, page_size)
     rows, cols = shape = q.shape
@@ -554,6 +554,11 @@ def _require_logits(logits: torch.Tensor, ids: torch.Tensor) -> tuple[int, int, 
     return rows, vocab, stride[0], dtype is not _BF16
 
 
+def _require_logprobs_workspace(workspace: torch.Tensor) -> None:
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor, got {workspace.dtype} strides {workspace.stride()}")
+
+
 def _require_logprobs_out(out: tuple[torch.Tensor, ...], rows: int, top: int) -> None:
     lp, ent, tid, tlp = out
     for name, t, dtype, shape in (("logprob", lp, torch.float32, (rows,)), ("entropy", ent, torch.float32, (rows,)),
@@ -566,7 +571,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out
                    workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
     """``(logprob, entropy, top_ids, top_logprobs)`` of ``logits [rows, vocab]`` (bf16 or fp32, any row stride): the log
     probability of ``ids [rows]``, the entropy (nats), and the ``top`` most likely tokens, largest first, of equal logits the
-    lower index first. Forbidden tokens are ``-inf``; a row of nothing else has log probabilities ``-inf`` and entropy 0."""
+    lower index first. Forbidden tokens are ``-inf`` (logits of ``-2**123`` and lower count as such beside higher ones); a row of
+    nothing else has log probabilities ``-inf`` and entropy 0."""
     rows, vocab, ld, fp32 = _require_logits(logits, ids)
     if out is None:
         out = token_logprobs_out(rows, top, logits.device)
@@ -574,6 +580,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, *, out
         _require_logprobs_out(out, rows, top)
     if workspace is None and rows > 0:
         workspace = token_logprobs_workspace(rows, vocab, top, logits.device)
+    elif workspace is not None:
+        _require_logprobs_workspace(workspace)
     idx = _same_device(logits, ids, workspace, *out)
     if rows == 0:
         return out
@@ -599,12 +607,13 @@ def token_logprobs_shard(logits: torch.Tensor, ids: torch.Tensor, vocab_start: i
     rows, vocab, ld, fp32 = _require_logits(logits, ids)
     if record.dtype != torch.uint8 or not record.is_contiguous() or record.numel() < int(_native.load().df_token_logprobs_record_bytes(rows, top)):
         raise ValueError("record must be a contiguous uint8 tensor from token_logprobs_record")
+    _require_logprobs_workspace(workspace)
     idx = _same_device(logits, ids, record, workspace)
     if rows == 0:
         return record
     _launch(idx, "df_token_logprobs_shard", logits.data_ptr(), fp32, ld, ids.data_ptr(),
             ids.element_size(), rows, vocab, vocab_start, top, record.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size())
+            workspace.nbytes)
     return record
 
 

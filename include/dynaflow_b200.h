@@ -510,7 +510,7 @@ int df_rope_append_paged4_bf16(const void* qkv, long long ld_qkv, void* out, lon
  * out, new_lens[b] of them (at most max_new are served; row_starts and new_lens as df_page_plan leaves them, or both
  * NULL: one row a request, row b); row j of them attends keys 0 .. seq_lens[b] - new_lens[b] + j, query head h reads
  * key/value head h / (q_heads / kv_heads). Keys whose page is missing (page_table outside [0, num_pages)) do not count;
- * a row without keys is zeros. Rows of no request are left as they were. `workspace`: device scratch of
+ * a row without keys is zeros; a length past what a row of the table holds is limited to that. Rows of no request are left as they were. `workspace`: device scratch of
  * df_attention_paged4_workspace_bytes(), whose first DF_ATTENTION_PAGED4_COUNTER_BYTES are zero before its first use (a
  * launch leaves them zero; after a status error zero them again); one for launches that can overlap. max_ctas limits
  * the launch to that many SMs (0: all). Reproducible bit for bit at a given max_ctas. */
@@ -527,7 +527,7 @@ int df_attention_paged4_bf16(const void* q, long long ld_q, const void* cache, c
  * Of rows of logits (bf16, or fp32 with fp32 = 1; any row stride ld >= vocab in elements): the log probability of the
  * row's given token (ids: int32 or int64 by id_bytes; an id outside the vocabulary gives -inf), the entropy in nats, and
  * the `top` (0 to 32) most likely tokens with their log probabilities, largest first, of equal logits the lower index
- * first. One pass over the logits; sums in fp32. Forbidden tokens are -inf; a row of nothing else has log probabilities
+ * first. One pass over the logits; sums in fp32. Forbidden tokens are -inf (logits of -2^123 and lower count as such beside higher ones); a row of nothing else has log probabilities
  * -inf and entropy 0; a row with a NaN or +inf gives NaN. `workspace` (df_token_logprobs_workspace_bytes, contents
  * arbitrary, one for launches that can overlap) holds the slices of rows. Deterministic. */
 size_t df_token_logprobs_workspace_bytes(int rows, int vocab, int top);

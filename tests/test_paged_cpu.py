@@ -204,3 +204,17 @@ def test_logprob_wrappers_refuse_wrong_tensors():
         ops.token_logprobs_shard(x, ids, 0, 2, torch.zeros(8, dtype=torch.uint8), torch.zeros(8, dtype=torch.uint8))
     with pytest.raises(ValueError, match="records"):
         ops.token_logprobs_join(torch.zeros(8, dtype=torch.uint8), 2, 2, 2)
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(64, dtype=torch.uint8)[::2],
+                                       torch.zeros(64, dtype=torch.float32)], ids=["expanded", "strided", "float"])
+def test_logprob_workspaces_are_what_their_size_says(workspace):
+    # the bytes of an expanded tensor's shape are not the bytes of its storage
+    from dynaflow_b200 import ops
+
+    x, ids = torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64)
+    record = torch.zeros(2 * (16 + 2 * 8), dtype=torch.uint8)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.token_logprobs(x, ids, 2, workspace=workspace)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.token_logprobs_shard(x, ids, 0, 2, record, workspace)
