@@ -197,3 +197,19 @@ def test_random_shapes(ops):
         x = (torch.randn(rows, vocab, generator=g) * rng.choice([0.1, 2.0, 10.0])).to(dtype)
         ids = torch.randint(0, vocab, (rows,), generator=g).tolist()
         _check(_run(ops, x.cuda(), ids, top), x, ids, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [31, 33, 255, 257, 534, 745, 1024, 1361, 1637, 2047, 2049, 8193, 8200, 17000])
+@pytest.mark.parametrize("top", [1, 7, 32])
+def test_rows_that_leave_warps_without_logits(ops, vocab, top, dtype):
+    # fewer vectors than threads, in the row or in its last slice: the threshold comes from the warps that have logits
+    top = min(top, vocab)
+    for rows in (3, 300):
+        g = torch.Generator().manual_seed(3 * vocab + rows)
+        logits = torch.randn(rows, vocab, generator=g).to(dtype)
+        logits[:, ::5] = -math.inf
+        ids = torch.randint(0, vocab, (rows,), generator=g).tolist()
+        got = _run(ops, logits.cuda(), ids, top)
+        some = slice(None, None, max(rows // 5, 1))
+        _check([t[some] for t in got], logits[some], ids[some], top)
