@@ -2,13 +2,21 @@
 //
 // A key is s_k n + m_k (16 code values n, one scale s_k and one minimum m_k a token and head), a value likewise:
 //   score(key) = scale * (s_k (q . n) + m_k sum(q))
-//   out        = (sum p s_v n_v + sum p m_v) / sum p,       p = exp(score - reference)
+//   out        = (sum p s_v (n_v - 7.5) + sum p (m_v + 7.5 s_v)) / sum p,       p = exp(score - reference)
 // so both products run on the codes themselves and the parameters are two multiplications a score.
 //
 // The codes feed the matrix instructions without a conversion: a 16-bit half with a code in its low four bits
 // is, read as fp16, the subnormal number n * 2^-24 (or 16 n * 2^-24 from the next four bits), which the
 // matrix units take exactly. Eight codes cost four ANDs and a shift. The powers of two are put back with the
-// scores and the result. Everything is summed in fp32; roundings to fewer bits:
+// scores and the result.
+//
+// The values are counted from the middle of their range because both sums of the result would otherwise grow with the
+// number of keys and all but cancel, and the matrix unit cuts its fp32 sums off instead of rounding them (about 2^-23 of
+// the sum a step, always towards zero): 65536 keys of N(0, 1) in one warp were 13 % off that way. Codes have no half steps
+// (and as fp16 numbers around zero they took an operation a pair, 26.0 us instead of 24.4 on 128 requests x 4096 tokens), so
+// keys 0-7 of a granule go in as n, keys 8-15 as -(15 - n): the complement of the word, and a weight with the other sign. That
+// is level where both halves weigh the same; what they do not is added up by a matrix instruction with rows of ones, and 7.5
+// times that is taken off the sums every LEVEL_TILES tiles. Everything is summed in fp32; roundings to fewer bits:
 //   * q is scaled by a power of two a row (its largest element to [2^14, 2^15)) and held in fp16: bf16 has 8
 //     significant bits, fp16 11, so only elements below 2^-28 of the largest lose any;
 //   * p s_v, scaled by a power of two so that it stays below 2^13, is held in fp16 for the value product: 2^-12
@@ -35,8 +43,8 @@
 //
 // Bound: HBM, 136 bytes a key and head: long caches stream at 6.3 TB/s (the difference between 65536 and 32768 tokens,
 // 8 requests, 8 heads: 285 MB in 45 us). Short ones are bound by what lies around that: about 5 us from the lengths
-// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 23.4 us.
-// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 74 us) a warp's chain of
+// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 24.4 us.
+// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 79 us) a warp's chain of
 // products and softmax is longer than its share of the bytes takes, at two warps a scheduler (228 registers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,6 +63,7 @@ constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padde
 constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
 constexpr int TILE = 2 * GRANULE;             // tokens
 constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
+constexpr int LEVEL_TILES = 8;                // tiles between two levellings of the sums (drafts of 4 tokens: 79.4 us; 4: 79.9, 2: 80.9, 1: 82.2)
 constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 33.9 us; 1: 39.5, 2: 34.4, 4: 33.8)
 constexpr unsigned JOIN_COST = 40;            // tiles of 8 columns a CTA does in the time that a join between CTAs takes
 constexpr int MAX_COLUMNS = 1 << 20;
@@ -465,8 +474,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   float c1[NT][2], sq[NT][2];                 // score = (acc s_k + sq m_k) c1, of columns 2t and 2t + 1
   int limit[NT][2];                           // keys a column sees
   float ref[NT][2], over[NT][2];              // reference (log2); a score that exceeds it by `over` moves it (-inf: none yet)
-  float l[NT][2], pm[NT][2];                  // sum p and sum p m_v, of this thread's keys
+  float l[NT][2], pm[NT][2];                  // sum p and sum p (m_v + 7.5 s_v), of this thread's keys
   float acc[NT][8][4];
+  float tilt[NT][4];                          // what keys 0-7 of the granules weigh more than keys 8-15, since acc was levelled
   float v_scale = 1.0f, v_limit = -1.0f;      // p s_v is held times v_scale = 2^-v_exp; scales above v_limit move it
   int v_exp = -100;
   int seg_b = -1, seg_hc = 0, seg_first = 0, seg_last = 0, min_limit = 0;
@@ -573,13 +583,30 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[nt][i][k] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tilt[nt][k] = 0.f;
       min_limit = min(min_limit, min(limit[nt][0], limit[nt][1]));
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, o));
   };
 
+  // Counts the codes of what is summed from 7.5: keys 0-7 stand there with n, keys 8-15 with n - 15.
+  auto level = [&]() {
+    constexpr float LO = 7.5f / 16777216.0f, HI = 16.0f * LO;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[nt][i][k] = fmaf(tilt[nt][k], k < 2 ? -LO : -HI, acc[nt][i][k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tilt[nt][k] = 0.f;
+    }
+  };
+
   auto flush = [&](bool last) {
+    level();
     const Weight w = weight(seg_b);
     const bool began = seg_first == 0, ended = seg_last == w.tiles - 1;
     int kvh, column0, row0;
@@ -776,6 +803,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
           }
         }
     }
+    // from here on the middle of a token's values instead of their minimum
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) vm[h][r] = fmaf(7.5f, vs[h][r], vm[h][r]);
     const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
     float top[NT][2];
     bool move = vmax > v_limit;
@@ -814,6 +846,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             acc[nt][i][c] *= both;
             acc[nt][i][2 + c] *= both;
           }
+          tilt[nt][c] *= both;
+          tilt[nt][2 + c] *= both;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             sc[h][nt][c] -= rise;
@@ -825,7 +859,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t pf[NT][2];
-      const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * v_scale};
+      const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * -v_scale};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
@@ -840,13 +874,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
         pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
+        mma_f16(tilt[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pf[nt][0], pf[nt][1]);
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         if (!EARLY) load_values(h, half);
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          const uint32_t x0 = vf[h][half][2 * cc], x1 = vf[h][half][2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+          const uint32_t x0 = vf[h][half][2 * cc], x1 = ~vf[h][half][2 * cc + 1], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_f16(acc[nt][4 * half + 2 * cc], code_lo(x0), code_hi(x0), code_lo(x1), code_hi(x1), pf[nt][0], pf[nt][1]);
@@ -855,6 +890,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         }
       }
     }
+    if ((n & (LEVEL_TILES - 1)) == LEVEL_TILES - 1) level();
     __syncwarp();  // every lane has read the stage
     const int next = n + STAGES;
     if (next < count) {

@@ -1,0 +1,85 @@
+"""How near the attention over the paged 4-bit cache comes to the 64-bit result, relative to the result's own size, where
+one warp walks a whole row of keys."""
+import pytest
+import torch
+
+from oracle import paged_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+HD, HEADS, PAGE = 128, 16, 64          # sixteen heads on one SM: one for each of its warps
+
+
+@pytest.fixture(scope="module")
+def ops(native_lib):
+    from dynaflow_b200 import ops as _ops
+
+    return _ops
+
+
+def _errors(ops, q, keys, values):
+    """``q [16, 128]`` (a key/value head each) against the same ``keys, values [n, 128]``: for every head the distance to the
+    64-bit result and its bound, both relative to the result's norm. The bound is the sum of
+    * the result's rounding to bf16, 2^-8;
+    * what the keys' weights are off by: the rounding of p s to fp16 (2^-11), and as derived for every row elsewhere, the score's
+      fp32 sum and exp2, 2 (2^-23 24 A + 2^-21), A the sum of the score's terms in magnitude. These errors are independent from
+      key to key, at most d each, so that their sum over the keys has a standard deviation of at most d sqrt(sum |p v|^2),
+      with the two parts of v, s (n - 7.5) and the middle m + 7.5 s, each on its own; four of them are allowed;
+    * the matrix unit's fp32 sums: at most two steps of 2^-23 of the largest partial sum for each 16 keys; in a sum there are also
+      the codes' means, 7.5, of what the halves of at most 512 keys' granules differ in weight;
+    * the fp32 sums of p and of p (m + 7.5 s): a lane adds n / 8 terms, half a step (2^-24) of the largest partial sum each,
+      independent: sqrt(n / 8) of them, four standard deviations."""
+    n = keys.shape[0]
+    data, kd, vd = oracle.pack_granules(keys, values)
+    codes, step, low = oracle.quantise(values)
+    pages = n // PAGE
+    cache = data.view(pages, 1, PAGE // 16, 2176).expand(pages, HEADS, PAGE // 16, 2176).contiguous().view(pages, HEADS, PAGE * 136).cuda()
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = torch.zeros(1, HEADS * HD, dtype=torch.bfloat16, device="cuda")
+    ops.attention_paged4(q.view(1, -1).cuda(), cache, table, lens, out, ops.attention_paged4_workspace(1, HEADS, HEADS), page_size=PAGE, max_ctas=1)
+    torch.cuda.synchronize()
+    ops.check_status()
+    got = out.cpu().double().view(HEADS, HD)
+    scale = HD ** -0.5
+    wave, middle = step * (codes - 7.5), low + 7.5 * step
+    found = []
+    for h in range(HEADS):
+        x = q[h].double()
+        p = torch.softmax(kd @ x * scale, 0)[:, None]
+        o = (p * vd).sum(0)
+        size = (x.abs().sum() * 2 * kd.abs().max() + (kd.abs() @ x.abs()).max()) * scale
+        each = 2.0 ** -11 + 2 * (2.0 ** -23 * 24 * size + 2.0 ** -21)
+        spread = ((p * wave).norm() ** 2 + HD * (p * middle).norm() ** 2).sqrt()
+        tilt = (p * step).view(-1, 2, 8).sum(2).diff(dim=1).view(-1, 32).cumsum(1).abs().max() * 2 * 7.5 * HD ** 0.5
+        cut = n / 16 * 2.0 ** -22 * ((p * wave).cumsum(0).abs().amax(0).norm() + tilt)
+        lane = 4 * (n / 8) ** 0.5 * 2.0 ** -24 * (HD ** 0.5 * (p * middle).cumsum(0).abs().max() + o.norm())
+        found.append(((got[h] - o).norm() / o.norm(), 2.0 ** -8 + (4 * each * spread + cut + lane) / o.norm()))
+    return torch.tensor(found, dtype=torch.float64)
+
+
+def _check(found):
+    assert torch.isfinite(found).all()
+    assert (found[:, 0] <= found[:, 1]).all(), found
+
+
+def _inputs(n, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(HEADS, HD, generator=g).bfloat16(), torch.randn(n, HD, generator=g), torch.randn(n, HD, generator=g))
+
+
+@pytest.mark.parametrize("n,shift", [(4096, 0.0), (16384, 0.0), (65536, 0.0), (65536, 3.0)])
+def test_long_rows_of_equal_keys(ops, n, shift):
+    """Results that shrink with the number of keys: nothing that grows with it may be left over."""
+    q, k, v = _inputs(n, n + int(shift))
+    _check(_errors(ops, q, k.bfloat16(), (v + shift).bfloat16()))
+
+
+def test_keys_that_count_in_one_half_of_every_sixteen(ops):
+    """The keys in places 8 to 15 of each granule have no weight."""
+    n = 65536
+    q, k, v = _inputs(n, 7)
+    base = torch.randn(HD, generator=torch.Generator().manual_seed(9))
+    q = (0.8 * base + 0.6 * q.float()).bfloat16()
+    k.view(-1, 16, HD)[:, 8:] -= 4 * base
+    _check(_errors(ops, q, k.bfloat16(), v.bfloat16()))
