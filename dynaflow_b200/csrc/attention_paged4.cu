@@ -19,8 +19,11 @@
 // times that is taken off the sums every LEVEL_TILES tiles. Everything is summed in fp32; roundings to fewer bits:
 //   * q is scaled by a power of two a row (its largest element to [2^14, 2^15)) and held in fp16: bf16 has 8
 //     significant bits, fp16 11, so only elements below 2^-28 of the largest lose any;
-//   * p s_v, scaled by a power of two so that it stays below 2^13, is held in fp16 for the value product: 2^-12
-//     of its value, against the 2^-9 of the bf16 result.
+//   * p s_v f is held in fp16 for the value product, f a power of two of each column that follows the largest p s_v seen so
+//     far and puts it near the upper end of the format: 2^11 when f is chosen, 2^15 at most. A weight is off by 2^-12 of its value
+//     (against the 2^-9 of the bf16 result), on codes of at most 7.5; where it is below 2^-25 of the largest, by 2^-36 of the
+//     largest. It does not follow s_v alone, nor the largest p: a key with most of the weight may have a value near zero,
+//     and a large value next to no weight, and what is left of the other keys is then the result.
 //
 // Both products are transposed, 16 keys on the rows of m16n8k16 and the query columns (new token x head of the
 // group) on its 8 columns:  S^T[16 keys, 8] = K[16, 128] Q^T  and  O^T[128 dims, 8] += V^T[128, 16 keys] P^T.
@@ -43,9 +46,9 @@
 //
 // Bound: HBM, 136 bytes a key and head: long caches stream at 6.3 TB/s (the difference between 65536 and 32768 tokens,
 // 8 requests, 8 heads: 285 MB in 45 us). Short ones are bound by what lies around that: about 5 us from the lengths
-// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 24.4 us.
-// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 79 us) a warp's chain of
-// products and softmax is longer than its share of the bytes takes, at two warps a scheduler (228 registers).
+// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 25.4 us.
+// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 81 us) a warp's chain of
+// products and softmax is longer than its share of the bytes takes, at two warps a scheduler (246 registers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -59,6 +62,9 @@ namespace paged {
 
 constexpr int WHERE_PAGED_ATTN = 51;
 constexpr float RESCALE_LIMIT = 8.0f;         // the reference moves when a score exceeds it by 2^8
+constexpr int WEIGHT_TOP = 11;                // the largest p s_v f when f is chosen: 2^11 at most,
+constexpr float WEIGHT_LIMIT = 15.0f;         // and never more than 2^15 (the largest fp16 number is 65504)
+constexpr int WEIGHT_SCALE_MAX = 100;         // f is at most 2^100: p f stays in fp32
 constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padded to 16 bytes
 constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
 constexpr int TILE = 2 * GRANULE;             // tokens
@@ -132,6 +138,10 @@ __device__ __forceinline__ float ex2f(float x) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
 __device__ __forceinline__ int exponent_of(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 0xffu) - 127; }
+// A whole number above log2 |x| by one at most: the biased exponent, put behind 2^23.
+__device__ __forceinline__ float above_log2(float x) { return __uint_as_float(((__float_as_uint(x) >> 23) & 0xffu) | 0x4b000000u) - (8388608.0f + 126.0f); }
+// 2^-x of a whole number x >= 0; 0 from 127 on.
+__device__ __forceinline__ float down(float x) { return x < 127.0f ? pow2i(-static_cast<int>(x)) : 0.0f; }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
@@ -477,8 +487,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
   float l[NT][2], pm[NT][2];                  // sum p and sum p (m_v + 7.5 s_v), of this thread's keys
   float acc[NT][8][4];
   float tilt[NT][4];                          // what keys 0-7 of the granules weigh more than keys 8-15, since acc was levelled
-  float v_scale = 1.0f, v_limit = -1.0f;      // p s_v is held times v_scale = 2^-v_exp; scales above v_limit move it
-  int v_exp = -100;
+  float f[NT][2], w_limit[NT][2];             // p s_v is held times f = 2^e; what exceeds 2^w_limit, w_limit = 15 - e, moves it
   int seg_b = -1, seg_hc = 0, seg_first = 0, seg_last = 0, min_limit = 0;
   Ends ends{-1, -1, 0, 0, -1, -1, count > 0 ? 1 : 0};
 
@@ -565,9 +574,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     place(w, b, hc, kvh, column0, row0);
     const int served = min(w.fresh, p.max_new);
     min_limit = w.len;
-    v_scale = 1.0f;
-    v_limit = -1.0f;
-    v_exp = -100;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -576,6 +582,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         limit[nt][k] = j < served ? min(w.len - w.fresh + j + 1, w.len) : w.len;  // a column without a query is computed and dropped
         ref[nt][k] = 0.f;
         over[nt][k] = -INFINITY;
+        f[nt][k] = pow2i(WEIGHT_SCALE_MAX);
+        w_limit[nt][k] = WEIGHT_LIMIT - WEIGHT_SCALE_MAX;
         l[nt][k] = 0.f;
         pm[nt][k] = 0.f;
       }
@@ -612,7 +620,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     int kvh, column0, row0;
     place(w, seg_b, seg_hc, kvh, column0, row0);
     const int served = min(w.fresh, p.max_new);
-    const float back = 16777216.0f * pow2i(v_exp);  // 2^24 of the codes
     float* part = nullptr;
     if (!began || !ended) {
       part = last ? reinterpret_cast<float*>(sm.ring[warp][0])  // every copy into the ring has been read
@@ -636,14 +643,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         const int j = div_small(c, p.inv_group), row = row0 + j;
         if (j >= served || row < 0 || row >= p.rows) continue;
         const float inv = part != nullptr ? 1.0f : (sum != 0.0f ? 1.0f / sum : 0.0f);  // no keys: zeros
-        const float f0 = back * inv, f1 = f0 * 0.0625f, more = add * inv;
+        const float back = pow2i(-exponent_of(f[nt][k])) * inv, more = add * inv;
         float* dst = part + local * PARTIAL_FLOATS;
         __nv_bfloat16* out = p.out + row * p.ld_out + (kvh * p.group + c - j * p.group) * HEAD_DIM;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
           // dimensions 32 c4 + 4 g .. + 3: rows g and g + 8 of m-tiles 2 c4 and 2 c4 + 1
-          const float o0 = fmaf(acc[nt][2 * c4][k], f0, more), o1 = fmaf(acc[nt][2 * c4][2 + k], f1, more);
-          const float o2 = fmaf(acc[nt][2 * c4 + 1][k], f0, more), o3 = fmaf(acc[nt][2 * c4 + 1][2 + k], f1, more);
+          constexpr float LO = 0x1p24f, HI = 0x1p20f;  // of the codes
+          const float o0 = fmaf(acc[nt][2 * c4][k] * LO, back, more), o1 = fmaf(acc[nt][2 * c4][2 + k] * HI, back, more);
+          const float o2 = fmaf(acc[nt][2 * c4 + 1][k] * LO, back, more), o3 = fmaf(acc[nt][2 * c4 + 1][2 + k] * HI, back, more);
           const int dim = 32 * c4 + 4 * g;
           if (part == nullptr) {
             const __nv_bfloat162 lo = __floats2bfloat162_rn(o0, o1), hi = __floats2bfloat162_rn(o2, o3);
@@ -808,46 +816,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r) vm[h][r] = fmaf(7.5f, vs[h][r], vm[h][r]);
-    const float vmax = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+    // What may move a column's references: a score above them, or a score and a scale (of one key, or so it is assumed here)
+    const float vmax = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+    const float vtop = above_log2(vmax);
     float top[NT][2];
-    bool move = vmax > v_limit;
+    bool move = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
-        move = move || top[nt][c] > over[nt][c];
+        move = move || top[nt][c] > fminf(over[nt][c], w_limit[nt][c] - vtop);
       }
     if (__any_sync(0xffffffffu, move)) {
-      // new references: the largest score of each column so far, the power of two above the largest scale so far
-      float most = vmax;
+      // new references: of p the largest score of each column so far, of p s_v f what the largest p s_v so far asks for. Both are
+      // whole powers of two, so that what is there moves to them without a rounding.
+      float ev[2][2];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const int e_new = max(v_exp, min(max(exponent_of(most) + 1, -100), 126));
-      const float beta = e_new == v_exp ? 1.0f : pow2i(max(v_exp - e_new, -126));
-      v_exp = e_new;
-      v_scale = pow2i(-e_new);
-      v_limit = pow2i(min(e_new + 4, 127));
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) ev[h][r] = above_log2(vs[h][r]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const bool none = over[nt][c] == -INFINITY;  // no key so far
-          const float high = max_rows(top[nt][c]), up = none ? high : fmaxf(high, 0.0f);
+          const float high = max_rows(top[nt][c]), up = ceilf(none ? high : fmaxf(high, 0.0f));
           const float rise = up != -INFINITY ? up : 0.0f;
-          const float alpha = none ? 1.0f : ex2f(-rise);
+          const float weighted = max_rows(fmaxf(fmaxf(sc[0][nt][c] + ev[0][0], sc[0][nt][2 + c] + ev[0][1]), fmaxf(sc[1][nt][c] + ev[1][0], sc[1][nt][2 + c] + ev[1][1])));
+          // f = 2^-e with the exponent that the sums now have, relative to the new reference, or a larger one
+          const float now = none ? -WEIGHT_SCALE_MAX : w_limit[nt][c] - WEIGHT_LIMIT - rise;
+          const float e = fmaxf(fmaxf(now, -WEIGHT_SCALE_MAX), ceilf(weighted - rise) - WEIGHT_TOP);
+          const float alpha = none ? 1.0f : down(rise), beta = none ? 1.0f : down(e - now);
           if (up != -INFINITY) over[nt][c] = RESCALE_LIMIT;
           ref[nt][c] += rise;
           l[nt][c] *= alpha;
           pm[nt][c] *= alpha;
-          const float both = alpha * beta;
+          f[nt][c] = pow2i(-static_cast<int>(e));
+          w_limit[nt][c] = WEIGHT_LIMIT + e;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            acc[nt][i][c] *= both;
-            acc[nt][i][2 + c] *= both;
+            acc[nt][i][c] *= beta;
+            acc[nt][i][2 + c] *= beta;
           }
-          tilt[nt][c] *= both;
-          tilt[nt][2 + c] *= both;
+          tilt[nt][c] *= beta;
+          tilt[nt][2 + c] *= beta;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             sc[h][nt][c] -= rise;
@@ -859,7 +872,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t pf[NT][2];
-      const float vsn[2] = {vs[h][0] * v_scale, vs[h][1] * -v_scale};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
@@ -868,7 +880,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
           const int r = k >> 1, c = k & 1;
           const float pr = ex2f(sc[h][nt][k]);
           l[nt][c] += pr;
-          w[k] = pr * vsn[r];
+          w[k] = pr * (r == 0 ? f[nt][c] : -f[nt][c]) * vs[h][r];
           pm[nt][c] = fmaf(pr, vm[h][r], pm[nt][c]);
         }
         const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
