@@ -33,6 +33,7 @@ namespace paged {
 // requests, a step and its return: 10.4 us), eight above (61 prompts, 125000 rows, and their return: 16.5 us).
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_REQUESTS = 8192;
+constexpr int plan_smem(int requests) { return 3 * (requests + 1) * static_cast<int>(sizeof(int)); }  // the prefix sums
 
 struct PlanParams {
   const int* lens;
@@ -424,17 +425,21 @@ extern "C" int df_page_plan(const int* seq_lens_dev, const int* new_lens_dev, in
   p.page_size = page_size;
   p.rows_per_request = rows_per_request;
   p.status = reinterpret_cast<Status*>(dev_status);
-  const int smem = 3 * (requests + 1) * static_cast<int>(sizeof(int));
+  // More than 48 KB (static part and all) a launch has to ask for: once a device, what the largest call needs.
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) {  // more than a launch has without asking
-    e = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan_smem(PLAN_MAX_REQUESTS));
     if (e != cudaSuccess) return fail(DF_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const int ctas = rows > 4 * PLAN_THREADS || requests > 2 * PLAN_THREADS ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, 1, 1);
   cfg.blockDim = dim3(PLAN_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = plan_smem(requests);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
