@@ -16,7 +16,8 @@ class PagedKVCache4:
     def __init__(self, layers: int, kv_heads: int, *, num_pages: int, page_size: int, max_requests: int, max_len: int,
                  max_rows: int, rope_theta: float = 10000.0, device: torch.device | str = "cuda") -> None:
         """``num_pages`` pages of ``page_size`` tokens in every layer, for at most ``max_requests`` requests of at most
-        ``max_len`` tokens and steps of at most ``max_rows`` rows."""
+        ``max_len`` tokens (in whole pages: what the last one holds past ``max_len`` can be used, a longer request is reported) and
+        steps of at most ``max_rows`` rows."""
         if layers <= 0 or max_requests <= 0 or max_len <= 0 or max_rows <= 0:
             raise ValueError("layers, max_requests, max_len and max_rows must be positive")
         self.page_size, self.kv_heads = page_size, kv_heads
@@ -29,7 +30,7 @@ class PagedKVCache4:
         self.row_starts = torch.zeros(max_requests + 1, **i32)
         self.slots = torch.full((max_rows,), -1, **i32)
         self.positions = torch.zeros(max_rows, **i32)
-        self.angles = ops.rope_angles(max_len, rope_theta, device)
+        self.angles = ops.rope_angles(self.page_table.shape[1] * page_size, rope_theta, device)   # whatever position a page gives a slot
 
     def plan(self, seq_lens: torch.Tensor, new_lens: torch.Tensor, rows_per_request: int = 0) -> None:
         """Pages, slots and positions of a step (``ops.page_plan``): ``seq_lens`` the requests' lengths after it, ``new_lens`` how
