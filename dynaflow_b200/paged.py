@@ -34,7 +34,8 @@ class PagedKVCache4:
 
     def plan(self, seq_lens: torch.Tensor, new_lens: torch.Tensor, rows_per_request: int = 0) -> None:
         """Pages, slots and positions of a step (``ops.page_plan``): ``seq_lens`` the requests' lengths after it, ``new_lens`` how
-        many of the tokens are new; a length of 0 gives a request's pages back."""
+        many of the tokens are new; a length of 0 gives a request's pages back. The new tokens' rows lie back to back, or request
+        ``b``'s from row ``b * rows_per_request`` on."""
         ops.page_plan(seq_lens, new_lens, self.page_table, self.page_counts, self.free_pages, self.free_count, self.row_starts,
                       self.slots, self.positions, page_size=self.page_size, rows_per_request=rows_per_request)
 
@@ -45,7 +46,12 @@ class PagedKVCache4:
                                page_size=self.page_size)
 
     def attend(self, layer: int, q: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor, seq_lens: torch.Tensor,
-               first_request: int = 0, max_ctas: int = 0) -> torch.Tensor:
-        """Attention of one new token a request: row ``i`` of ``q`` is request ``first_request + i``."""
-        table = self.page_table[first_request:first_request + seq_lens.shape[0]]
-        return ops.attention_paged4(q, self.layers[layer], table, seq_lens, out, workspace, page_size=self.page_size, max_ctas=max_ctas)
+               first_request: int = 0, max_ctas: int = 0, *, new_lens: torch.Tensor | None = None, max_new: int = 1) -> torch.Tensor:
+        """Attention of the new tokens of requests ``first_request ...`` (as many as ``seq_lens``, their lengths, has). Without
+        ``new_lens`` row ``i`` of ``q`` is the last token of request ``first_request + i``, as a plan with ``rows_per_request=1`` lays a
+        step out. With ``new_lens``, the plan's of these requests, ``q`` and ``out`` are all of the step's rows, and a request's, at most
+        ``max_new``, are where the plan put them: any other layout needs it, since a request without a new token has no row there."""
+        requests = slice(first_request, first_request + seq_lens.shape[0])
+        starts = None if new_lens is None else self.row_starts[requests.start:requests.stop + 1]
+        return ops.attention_paged4(q, self.layers[layer], self.page_table[requests], seq_lens, out, workspace, page_size=self.page_size,
+                                    max_ctas=max_ctas, row_starts=starts, new_lens=new_lens, max_new=max_new)
