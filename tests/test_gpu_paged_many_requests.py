@@ -1,12 +1,16 @@
 """The paged operators with thousands of requests."""
 import os
+import random
 import subprocess
 import sys
 import textwrap
 
 import pytest
+import test_gpu_paged_attention as attention
+import torch
 
 from conftest import ROOT
+from dynaflow_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +57,24 @@ def test_plan_of_thousands_of_requests_first_in_its_process(native_lib, tmp_path
     script.write_text(PLAN_WORKER.format(root=ROOT, sizes=sizes))
     r = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=240, cwd=ROOT, env=dict(os.environ))
     assert r.returncode == 0 and "PLANS_OK" in r.stdout, r.stdout[-1000:] + r.stderr[-2000:]
+
+
+# more requests than have their lengths and prefix sums in shared memory (1024), around that number and odd
+@pytest.mark.parametrize("requests,max_ctas", [(1024, 0), (1025, 0), (1025, 3), (3001, 0), (3001, 1)])
+@pytest.mark.parametrize("several", [False, True])
+def test_attention_of_thousands_of_requests(native_lib, requests, max_ctas, several):
+    """Empty requests, one token, several pages; one long one, which is cut; with several new tokens some without any."""
+    rng = random.Random(requests + max_ctas)
+    lens = [rng.choice([0, 1, 15, 16, 17, 40]) for _ in range(requests)]
+    lens[requests // 3] = 1500
+    case = attention.Case(lens, 1, 16, requests)
+    fresh = [min(n, rng.choice([0, 1, 1, 2, 3])) for n in lens] if several else [1] * requests
+    starts = [sum(fresh[:b]) for b in range(requests + 1)] if several else list(range(requests + 1))
+    rows = starts[-1] + (3 if several else 0)
+    q = torch.randn(rows, 4 * 128, generator=torch.Generator().manual_seed(requests)).bfloat16()
+    more = dict(fresh=fresh, starts=starts, max_new=3) if several else {}
+    got = attention._run(ops, case, q, 4, max_ctas=max_ctas, **more)
+    want, tol = attention._want(case, q, starts, fresh, 4, 128 ** -0.5)
+    served = torch.zeros(rows, dtype=torch.bool)
+    served[:starts[-1]] = True
+    attention._check(got, want, tol, served)
