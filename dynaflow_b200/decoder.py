@@ -104,19 +104,18 @@ class TensorParallelDecoder:
         self.gemm_max_ctas = gemm_max_ctas                    # CTAs the GEMMs may use (0 = one per SM)
         self.launch_count = 0
         self.paged: PagedKVCache4 | None = None               # init_decode_paged: the cache in pages of 4-bit codes
-        self._prefill_paged = False
 
     # ------------------------------------------------------------------ pieces
     def _partial(self, mb: int, rows: int) -> torch.Tensor:
         return self.comm.partial(mb, rows) if self.comm is not None else self.partial_local[mb][:rows]
 
     def _attention_half(self, layer: dict, x: torch.Tensor, mb: int, batch: int, seq: int, pos: torch.Tensor, li: int = 0,
-                        first_row: int = 0) -> None:
+                        first_row: int = 0, paged: bool = False) -> None:
         s = self.s
         rows = batch * seq
         qkv = self.qkv[mb][:rows]
         ops.gemm_bf16(x, layer["wqkv"], out=qkv, max_ctas=self.gemm_max_ctas)
-        if self._prefill_paged:      # the keys and values come back as the cache holds them: what later steps will see
+        if paged:                    # the keys and values come back as the cache holds them: what later steps will see
             self.paged.append(li, qkv, self.qh, first_row)
         else:
             rc = self.lib.df_rope_bf16(qkv.data_ptr(), pos.data_ptr(), rows, self.qh + self.kvh, s.head_dim, qkv.stride(0),
@@ -152,6 +151,9 @@ class TensorParallelDecoder:
         as per-micro-batch views concatenated. Requests are cut evenly into micro-batches.
         ``skip_comm`` / ``skip_compute`` leave out the reductions, resp. the GEMMs and attention
         (timing of the two halves of the overlap; the values are then meaningless)."""
+        return self._forward(ids, skip_comm, skip_compute)
+
+    def _forward(self, ids: torch.Tensor, skip_comm: bool = False, skip_compute: bool = False, paged: bool = False) -> torch.Tensor:
         s = self.s
         batch, seq = ids.shape
         n = min(self.micro_batches, batch)
@@ -202,7 +204,7 @@ class TensorParallelDecoder:
                     main.wait_event(done[mb])
                 b, rows = rows_of[mb]
                 if not skip_compute:
-                    self._attention_half(layer, xs[mb], mb, b, seq, pos[:rows], li, cuts[mb] * seq)
+                    self._attention_half(layer, xs[mb], mb, b, seq, pos[:rows], li, cuts[mb] * seq, paged)
                 reduce_after(mb, layer["norm2"])
             nxt = self.layers[li + 1]["norm1"] if li + 1 < len(self.layers) else self.final_norm
             for mb in range(n):
@@ -279,11 +281,7 @@ class TensorParallelDecoder:
             raise ValueError("prefill_paged needs init_decode_paged for this batch, and rows for all of its tokens")
         self.seq_lens.fill_(seq)
         self.paged.plan(self.seq_lens, torch.full_like(self.seq_lens, seq), rows_per_request=seq)
-        self._prefill_paged = True
-        try:
-            return self.forward(ids)
-        finally:
-            self._prefill_paged = False
+        return self._forward(ids, paged=True)
 
     def _attention_half_decode(self, li: int, layer: dict, x: torch.Tensor, mb: int) -> None:
         """qkv projection, RoPE at the sequences' last positions, the new keys and values into the

@@ -1,4 +1,4 @@
-"""Sequences that grow past the length the paged cache was made for."""
+"""The decoder over the paged cache: sequences that grow past the length it was made for, and a forward pass during a prefill."""
 import pytest
 import torch
 
@@ -38,3 +38,31 @@ def test_steps_past_max_len_inside_the_last_page(native_lib):
         with pytest.raises(ops.DeviceStatusError, match="table row full"):
             ops.check_status()
     assert torch.isfinite(runs[0].float()).all() and torch.equal(runs[0], runs[1])
+
+
+def test_a_forward_pass_during_a_prefill_leaves_the_pages_alone(native_lib):
+    """Whether keys and values go into the pages is the call's, not the object's: a forward pass that another thread starts
+    while prompts are brought in does not append."""
+    import threading
+
+    from dynaflow_b200 import ops
+
+    B, S = 2, 20
+    shape, dec = _decoder(B, S)
+    ids = torch.randint(0, shape.vocab, (B, S), generator=torch.Generator().manual_seed(8)).cuda()
+    dec.init_decode_paged(B, 32, page_size=16)
+    append, calls = dec.paged.append, []
+
+    def counted(*args):
+        calls.append(threading.current_thread())
+        if len(calls) == 1:
+            other = threading.Thread(target=dec.forward, args=(ids,))
+            other.start()
+            other.join()
+        append(*args)
+
+    dec.paged.append = counted
+    dec.prefill_paged(ids)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert len(calls) == shape.layers * 2 and set(calls) == {threading.current_thread()}
