@@ -140,8 +140,6 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 __device__ __forceinline__ int exponent_of(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 0xffu) - 127; }
 // A whole number above log2 |x| by one at most: the biased exponent, put behind 2^23.
 __device__ __forceinline__ float above_log2(float x) { return __uint_as_float(((__float_as_uint(x) >> 23) & 0xffu) | 0x4b000000u) - (8388608.0f + 126.0f); }
-// 2^-x of a whole number x >= 0; 0 from 127 on.
-__device__ __forceinline__ float down(float x) { return x < 127.0f ? pow2i(-static_cast<int>(x)) : 0.0f; }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
@@ -829,8 +827,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
         move = move || top[nt][c] > fminf(over[nt][c], w_limit[nt][c] - vtop);
       }
     if (__any_sync(0xffffffffu, move)) {
-      // new references: of p the largest score of each column so far, of p s_v f what the largest p s_v so far asks for. Both are
-      // whole powers of two, so that what is there moves to them without a rounding.
+      // new references: of p the largest score of each column so far, of p s_v f what the largest p s_v so far asks for. f stays a
+      // whole power of two: the largest p is 1, and its weight is not rounded.
       float ev[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -841,13 +839,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const bool none = over[nt][c] == -INFINITY;  // no key so far
-          const float high = max_rows(top[nt][c]), up = ceilf(none ? high : fmaxf(high, 0.0f));
+          const float high = max_rows(top[nt][c]), up = none ? high : fmaxf(high, 0.0f);
           const float rise = up != -INFINITY ? up : 0.0f;
           const float weighted = max_rows(fmaxf(fmaxf(sc[0][nt][c] + ev[0][0], sc[0][nt][2 + c] + ev[0][1]), fmaxf(sc[1][nt][c] + ev[1][0], sc[1][nt][2 + c] + ev[1][1])));
-          // f = 2^-e with the exponent that the sums now have, relative to the new reference, or a larger one
+          // f = 2^-e, no smaller an exponent than the sums now have relative to the new reference
           const float now = none ? -WEIGHT_SCALE_MAX : w_limit[nt][c] - WEIGHT_LIMIT - rise;
-          const float e = fmaxf(fmaxf(now, -WEIGHT_SCALE_MAX), ceilf(weighted - rise) - WEIGHT_TOP);
-          const float alpha = none ? 1.0f : down(rise), beta = none ? 1.0f : down(e - now);
+          const float e = ceilf(fmaxf(fmaxf(now, -WEIGHT_SCALE_MAX), weighted - rise - WEIGHT_TOP));
+          const float alpha = none ? 1.0f : ex2f(-rise), beta = none ? 1.0f : ex2f(now - e);
           if (up != -INFINITY) over[nt][c] = RESCALE_LIMIT;
           ref[nt][c] += rise;
           l[nt][c] *= alpha;

@@ -128,3 +128,19 @@ def test_values_near_the_end_of_the_range(ops):
     q, k, v = _inputs(4096, 6)
     _check(_errors(ops, q, k.bfloat16(), (v * 2.0 ** 120).bfloat16()))
     _check(_errors(ops, q, k.bfloat16(), (v * 2.0 ** -100).bfloat16()))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_one_key_with_all_of_the_weight_gives_its_value(ops, n):
+    """The largest weight is 1 and is not rounded: the result is the value's numbers, s n + m, rounded once. (They and the middle
+    m + 7.5 s fit into fp32: 8 bits each, 15 / 2 times at most, and the exponents are close.)"""
+    q, k, v = _inputs(48, 11)
+    k[n - 1] = 40 * q[0].float()
+    k, v = k.bfloat16(), v.bfloat16()
+    data, _, vd = oracle.pack_granules(k, v)
+    out = torch.zeros(1, 4 * HD, dtype=torch.bfloat16, device="cuda")
+    ops.attention_paged4(q[:1].repeat(1, 4).cuda(), data.view(1, 1, 48 * 136).cuda(), torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                         torch.tensor([n], dtype=torch.int32, device="cuda"), out, ops.attention_paged4_workspace(1, 4, 1), page_size=48)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert torch.equal(out.cpu().view(4, HD), vd[n - 1].bfloat16().expand(4, HD))
