@@ -13,7 +13,7 @@
 // The values are counted from the middle of their range because both sums of the result would otherwise grow with the
 // number of keys and all but cancel, and the matrix unit cuts its fp32 sums off instead of rounding them (about 2^-23 of
 // the sum a step, always towards zero): 65536 keys of N(0, 1) in one warp were 13 % off that way. Codes have no half steps
-// (and as fp16 numbers around zero they took an operation a pair, 26.0 us instead of 24.4 on 128 requests x 4096 tokens), so
+// (and made into fp16 numbers around zero, one operation a pair, they cost 1.6 us more on 128 requests x 4096 tokens), so
 // keys 0-7 of a granule go in as n, keys 8-15 as -(15 - n): the complement of the word, and a weight with the other sign. That
 // is level where both halves weigh the same; what they do not is added up by a matrix instruction with rows of ones, and 7.5
 // times that is taken off the sums every LEVEL_TILES tiles. Everything is summed in fp32; roundings to fewer bits:
@@ -44,10 +44,11 @@
 // A request and head costs a warp its queries and its result as well as its tiles, so it counts SEGMENT_COST tiles
 // more when the list is cut (without: 16 requests of a few tokens among long ones make one CTA twice as long).
 //
-// Bound: HBM, 136 bytes a key and head: long caches stream at 6.3 TB/s (the difference between 65536 and 32768 tokens,
-// 8 requests, 8 heads: 285 MB in 45 us). Short ones are bound by what lies around that: about 5 us from the lengths
-// over the page table to the first data, 3 to 8 us of joins. 128 requests x 4096 tokens, one head: 71 MB in 25.4 us.
-// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 81 us) a warp's chain of
+// Bound: HBM, 136 bytes a key and head, with the instructions close behind: long caches stream at 5.6 TB/s (the difference
+// between 65536 and 32768 tokens, 8 requests, 8 heads: 285 MB in 51 us), where a scheduler issues in every second cycle. Short
+// ones are bound by what lies around that: about 5 us from the lengths over the page table to the first data, 3 to 8 us of
+// joins. 128 requests x 4096 tokens, one head: 71 MB in 25.4 us.
+// With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 82 us) a warp's chain of
 // products and softmax is longer than its share of the bytes takes, at two warps a scheduler (246 registers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -69,8 +70,8 @@ constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padde
 constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
 constexpr int TILE = 2 * GRANULE;             // tokens
 constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
-constexpr int LEVEL_TILES = 8;                // tiles between two levellings of the sums (drafts of 4 tokens: 79.4 us; 4: 79.9, 2: 80.9, 1: 82.2)
-constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 33.9 us; 1: 39.5, 2: 34.4, 4: 33.8)
+constexpr int LEVEL_TILES = 8;                // tiles between two levellings of the sums (4 new tokens: 81.6 us; 16: 81.3, 4: 82.1, 1: 85.2)
+constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 35.7 us; 1: 41.0, 2: 35.7, 4: 35.8)
 constexpr unsigned JOIN_COST = 40;            // tiles of 8 columns a CTA does in the time that a join between CTAs takes
 constexpr int MAX_COLUMNS = 1 << 20;
 
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     if (cost > 0) {
       const Cut cut = cut_of(cost);
       // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
-      // head, on 148 CTAs: 23.4 us against 26.2 us cut evenly)
+      // head, on 148 CTAs: 25.4 us against 27.5 us cut evenly)
       per_cta = (all.y + gridDim.x - 1) / gridDim.x;
       whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
       parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;
