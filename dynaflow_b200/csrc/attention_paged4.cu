@@ -44,10 +44,10 @@
 // A request and head costs a warp its queries and its result as well as its tiles, so it counts SEGMENT_COST tiles
 // more when the list is cut (without: 16 requests of a few tokens among long ones make one CTA twice as long).
 //
-// Bound: HBM, 136 bytes a key and head, with the instructions close behind: long caches stream at 5.6 TB/s (the difference
-// between 65536 and 32768 tokens, 8 requests, 8 heads: 285 MB in 51 us), where a scheduler issues in every second cycle. Short
+// Bound: HBM, 136 bytes a key and head, with the instructions close behind: long caches stream at 5.8 TB/s (the difference
+// between 65536 and 32768 tokens, 8 requests, 8 heads: 285 MB in 49 us), where a scheduler issues in about every second cycle. Short
 // ones are bound by what lies around that: about 5 us from the lengths over the page table to the first data, 3 to 8 us of
-// joins. 128 requests x 4096 tokens, one head: 71 MB in 25.4 us.
+// joins. 128 requests x 4096 tokens, one head: 71 MB in 24.8 us.
 // With 9 to 16 columns (4 new tokens of 4 heads, 5 requests of 20000 to 65536 tokens: 244 MB in 82 us) a warp's chain of
 // products and softmax is longer than its share of the bytes takes, at two warps a scheduler (246 registers).
 #include <cuda_bf16.h>
@@ -70,8 +70,8 @@ constexpr int PARTIAL_FLOATS = HEAD_DIM + 4;  // O, reference (log2), sum; padde
 constexpr int REQUESTS_IN_SMEM = 1024;        // requests whose lengths and prefix sums fit into shared memory
 constexpr int TILE = 2 * GRANULE;             // tokens
 constexpr int TILE_BYTES = 2 * GRANULE_BYTES;
-constexpr int LEVEL_TILES = 8;                // tiles between two levellings of the sums (4 new tokens: 81.6 us; 16: 81.3, 4: 82.1, 1: 85.2)
-constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 35.7 us; 1: 41.0, 2: 35.7, 4: 35.8)
+constexpr int LEVEL_TILES = 8;                // tiles between two levellings of the sums (4 new tokens: 81.9 us; 16: 81.6, 4: 82.2, 1: 83.9)
+constexpr unsigned SEGMENT_COST = 3;          // tiles (48 requests of 1 to 16384 tokens, 8 heads: 35.0 us; 1: 39.9, 2: 35.1, 4: 35.2)
 constexpr unsigned JOIN_COST = 40;            // tiles of 8 columns a CTA does in the time that a join between CTAs takes
 constexpr int MAX_COLUMNS = 1 << 20;
 
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
     if (cost > 0) {
       const Cut cut = cut_of(cost);
       // Whole segments a CTA where that costs less than the joins that it saves (128 requests of 4096 tokens, one key/value
-      // head, on 148 CTAs: 25.4 us against 27.5 us cut evenly)
+      // head, on 148 CTAs: 24.8 us against 27.3 us cut evenly)
       per_cta = (all.y + gridDim.x - 1) / gridDim.x;
       whole = per_cta * (longest + SEGMENT_COST) <= cut.each + JOIN_COST / NT;
       parts = whole ? (all.y + per_cta - 1) / per_cta : cut.parts;
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[nt][i][k] = fmaf(tilt[nt][k], k < 2 ? -LO : -HI, acc[nt][i][k]);
+        for (int k = 0; k < 4; ++k) acc[nt][i][k] = fmaf(tilt[nt][k & 1], k < 2 ? -LO : -HI, acc[nt][i][k]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) tilt[nt][k] = 0.f;
     }
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged4_kernel(const A
             acc[nt][i][2 + c] *= beta;
           }
           tilt[nt][c] *= beta;
-          tilt[nt][2 + c] *= beta;
+          tilt[nt][2 + c] = 0.f;  // the rows are all alike, these are not read
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             sc[h][nt][c] -= rise;
